@@ -622,6 +622,110 @@ H3B200_API int h3b200_tp_gated_mlp(void* comm, const void* x, int64_t ldx, const
                                    const float* s2, void* out, int64_t ldo, int64_t m, int64_t chunk_rows,
                                    h3b200_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Attention after the Q/K/V build. 16-bit elements: dtype H3B200_DTYPE_BF16 or
+ * H3B200_DTYPE_F16, one for all tensors of a call. head_dim is 128. Strides are in
+ * elements, multiples of 8; the head dim is contiguous and rows are 16-byte
+ * aligned. Sums, softmax statistics, norms and rotations are fp32 (block means and
+ * their products 64-bit); results are rounded once, when they are stored.
+ * The reference runs attention through external libraries (kernels.py:7637); these
+ * entry points have no counterpart in it.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * Appends `tokens` keys and values to a paged cache, with per-head RMSNorm and
+ * split-half rotation of K, and of Q beside it, on the way:
+ *   h = x / sqrt(mean(x^2) + eps) * w   (w NULL: h = x);  rotation of the first rot_dim
+ *   dims as h3b200_qknorm_rope_strided;  K and V go to row slot % page_size of page
+ *   slot / page_size, Q to q_out.
+ * k, v: [tokens, kv_heads, 128], q, q_out: [tokens, heads, 128] (q NULL: no Q; q_out may
+ * be q). k_cache, v_cache: [pages, kv_heads, page_size, 128] at page / head / row
+ * strides. slots: int64 (slots_dtype 1) or int32 (0) per token; a token whose slot
+ * lies outside [0, pages * page_size), e.g. -1, is padding: nothing of it is written, its
+ * q_out row included. Slots of one call must differ: which token a shared slot
+ * ends up with is not defined. freqs: rows [rot_dim / 2, 2, 2] of freqs_dtype (as
+ * h3b200_qknorm_rope_strided) at stride f_st; token t uses row positions[t]
+ * (positions_dtype like slots_dtype), or t where positions is NULL; a position outside
+ * [0, freqs_rows) gives NaN in the rotated dims. freqs NULL or rot_dim 0: no rotation.
+ * rot_dim: a multiple of 16, at most 128.
+ */
+H3B200_API int h3b200_append_paged_kv(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st,
+                                      int64_t qo_sh, const void* q_weight, const void* k, int64_t k_st, int64_t k_sh,
+                                      const void* k_weight, const void* v, int64_t v_st, int64_t v_sh, void* k_cache,
+                                      int64_t kc_sp, int64_t kc_sh, int64_t kc_sr, void* v_cache, int64_t vc_sp,
+                                      int64_t vc_sh, int64_t vc_sr, int64_t pages, int64_t page_size,
+                                      const void* slots, int slots_dtype, const void* positions, int positions_dtype,
+                                      const void* freqs, int freqs_dtype, int64_t freqs_rows, int64_t f_st,
+                                      int64_t rot_dim, float eps, int dtype, int64_t tokens, int64_t heads,
+                                      int64_t kv_heads, h3b200_stream_t stream);
+
+/*
+ * Attention of one new token per sequence over a paged cache:
+ *   out[b, h] = sum_j softmax_j(scale q[b, h] . k_j) v_j over the keys j < lengths[b],
+ *   lse[b, h] = ln sum_j exp(scale q[b, h] . k_j)     (lse NULL: not written)
+ * with key j in row j % page_size of page page_table[b, j / page_size]; query head h reads
+ * key head h / (heads / kv_heads). lengths (int32) are clamped to [0, table_width *
+ * page_size]; a sequence without keys gives 0 and lse = -inf. Page ids outside
+ * [0, pages) hold no keys (nothing is read). Rows behind a sequence's last key are not
+ * read into the result, whatever they hold. page_size: a multiple of 8. page_table:
+ * int32 [batch, table_width] at stride pt_sb. out, lse strides as given.
+ * workspace: h3b200_paged_decode_workspace_bytes (which depends on the current device's SM
+ * count) bytes, 256-byte aligned; not needed after the call's work has run.
+ * The same inputs give the same bits on every call.
+ */
+H3B200_API int64_t h3b200_paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                                       int64_t table_width, int64_t page_size);
+H3B200_API int h3b200_paged_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache,
+                                             int64_t kc_sp, int64_t kc_sh, int64_t kc_sr, const void* v_cache,
+                                             int64_t vc_sp, int64_t vc_sh, int64_t vc_sr, int64_t pages,
+                                             int64_t page_size, const int32_t* page_table, int64_t pt_sb,
+                                             int64_t table_width, const int32_t* lengths, void* out, int64_t o_sb,
+                                             int64_t o_sh, float* lse, int64_t l_sb, int64_t l_sh, int64_t batch,
+                                             int64_t heads, int64_t kv_heads, float scale, int dtype, void* workspace,
+                                             int64_t workspace_bytes, h3b200_stream_t stream);
+
+/*
+ * Means of the blocks of x [tokens, heads, 128]: fp32 [heads, ceil(tokens / block), 128],
+ * summed in 64 bits and rounded once; the last block's mean covers the rows it has.
+ */
+H3B200_API int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t x_sh, int64_t tokens, int64_t heads,
+                                            int64_t block, int dtype, float* means, h3b200_stream_t stream);
+
+/*
+ * Key blocks that block-sparse attention reads, from block means of queries (blocks of
+ * 128) and keys (blocks of `block`):
+ *   score[i, j] = sum over the heads h of the group of q_means[h, i] . k_means[kv_head, j]  (64 bits)
+ * blocks[kv_head, i]: the top_k highest scores' j in ascending order (equal scores: the
+ * lowest j; NaN below every number), -1 behind them when fewer blocks can be seen.
+ * causal: query row r stands at position r + keys - queries. Key blocks that start
+ * behind the query block's last position are never selected; those that hold a
+ * position at or behind its first one come before all others.
+ */
+H3B200_API int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t heads, int64_t kv_heads,
+                                        int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
+                                        int32_t* blocks, h3b200_stream_t stream);
+
+/*
+ * Attention of query blocks of 128 rows over listed key blocks:
+ *   out[r, h] = sum_j softmax_j(scale q[r, h] . k_j) v_j,  lse[r, h] = ln sum_j exp(scale q[r, h] . k_j)
+ * over the keys j of blocks[h / (heads / kv_heads), r / 128, :] (int32, contiguous [kv_heads,
+ * ceil(queries / 128), top_k]; ids outside the keys' blocks name none, an id named twice
+ * counts twice), with causal those at positions <= r + keys - queries. A row that sees no
+ * key gives 0 and lse = -inf. block: 64 or 128 keys. Values of a tile that some row of a
+ * query block may not see (causal) still enter its products with weight zero, so they
+ * must be finite; rows behind the last key do not exist for the kernel. q, k, v, out:
+ * [tokens, heads, 128] at token / head strides. scale > 0.
+ */
+H3B200_API int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads,
+                                                       int64_t top_k, int64_t block);
+H3B200_API int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                             int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh,
+                                             const int32_t* blocks, int64_t top_k, int64_t block, void* out,
+                                             int64_t o_st, int64_t o_sh, float* lse, int64_t l_st, int64_t l_sh,
+                                             int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
+                                             float scale, int causal, int dtype, void* workspace,
+                                             int64_t workspace_bytes, h3b200_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

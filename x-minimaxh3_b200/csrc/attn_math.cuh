@@ -1,0 +1,62 @@
+// 16-bit element arithmetic shared by the attention kernels: bf16 or fp16
+// storage, fp32 values, packed pairs in 32-bit words (low half first).
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace h3 {
+
+constexpr int kHeadDim = 128;  // the head dim of every attention kernel of this library
+
+template <bool F16>
+struct Elem16 {
+  static __device__ __forceinline__ float lo(uint32_t w) {
+    if constexpr (F16) return __half2float(__ushort_as_half((unsigned short)(w & 0xFFFFu)));
+    return bf16_lo(w);
+  }
+  static __device__ __forceinline__ float hi(uint32_t w) {
+    if constexpr (F16) return __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+    return bf16_hi(w);
+  }
+  // two floats -> packed pair, each rounded to nearest even
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    if constexpr (F16) {
+      uint32_t r;
+      asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+      return r;
+    }
+    return pack_bf16(lo, hi);
+  }
+  // c[16 x 8] += a[16 x 16] b[16 x 8], fp32 sums
+  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    if constexpr (F16)
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+      asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                   : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+};
+
+// transpose of an 8 x 8 matrix of 16-bit values held one row per four lanes
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t w) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
+  return r;
+}
+
+// 128-bit read-only load of data this SM reads once (no L1 line kept)
+__device__ __forceinline__ uint4 ldg_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+}  // namespace h3

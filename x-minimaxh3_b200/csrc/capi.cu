@@ -11,6 +11,7 @@
 #include <mutex>
 #include <string>
 
+#include "attn_math.cuh"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -1412,5 +1413,189 @@ int h3b200_tp_gated_mlp(void* comm, const void* x, int64_t ldx, const void* resi
   return tp_stage_impl(c, 4, last, x, ldx, residual, ldr, gate, w1q, s1, w2q, s2, out, ldo, prev_lo, prev_hi, st);
 }
 
-}  // extern "C"
+// ---- attention after the Q/K/V build -----------------------------------------
 
+namespace {
+
+int attn_dtype(int dtype, const char* who) {
+  if (dtype == H3B200_DTYPE_BF16 || dtype == H3B200_DTYPE_F16) return H3B200_OK;
+  return fail(H3B200_ERR_INVALID, "%s: dtype code must be 1 (float16) or 2 (bfloat16), got %d", who, dtype);
+}
+
+int attn_heads(int64_t heads, int64_t kv_heads, const char* who) {
+  if (heads > 0 && kv_heads > 0 && heads % kv_heads == 0 && heads <= 65536) return H3B200_OK;
+  return fail(H3B200_ERR_INVALID, "%s: heads %lld must be a positive multiple of kv_heads %lld (at most 65536)", who, (long long)heads, (long long)kv_heads);
+}
+
+int current_sms() {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+  return h3::num_sms(dev);
+}
+
+// page sizes are multiples of 8 keys; key indices of one sequence are 32-bit
+int paged_shape(int64_t pages, int64_t page_size, const char* who) {
+  if (pages >= 0 && page_size > 0 && page_size % 8 == 0 && page_size <= (1 << 20)) return H3B200_OK;
+  return fail(H3B200_ERR_INVALID, "%s: page_size must be a positive multiple of 8 (got %lld) and pages >= 0 (got %lld)", who, (long long)page_size, (long long)pages);
+}
+
+}  // namespace
+
+int h3b200_append_paged_kv(const void* q, int64_t q_st, int64_t q_sh, void* q_out, int64_t qo_st, int64_t qo_sh,
+                           const void* q_weight, const void* k, int64_t k_st, int64_t k_sh, const void* k_weight,
+                           const void* v, int64_t v_st, int64_t v_sh, void* k_cache, int64_t kc_sp, int64_t kc_sh,
+                           int64_t kc_sr, void* v_cache, int64_t vc_sp, int64_t vc_sh, int64_t vc_sr, int64_t pages,
+                           int64_t page_size, const void* slots, int slots_dtype, const void* positions,
+                           int positions_dtype, const void* freqs, int freqs_dtype, int64_t freqs_rows, int64_t f_st,
+                           int64_t rot_dim, float eps, int dtype, int64_t tokens, int64_t heads, int64_t kv_heads,
+                           h3b200_stream_t stream) {
+  H3_GUARD("append_paged_kv", stream);
+  const char* who = "append_paged_kv";
+  if (const int rc = attn_dtype(dtype, who)) return rc;
+  if (const int rc = paged_shape(pages, page_size, who)) return rc;
+  if (tokens < 0 || kv_heads <= 0 || kv_heads > 65536 || (q && (heads <= 0 || heads > 65536)) || freqs_rows < 0 || f_st < 0) return fail(H3B200_ERR_INVALID, "%s: bad shape", who);
+  const int64_t rot = freqs ? rot_dim : 0;
+  if (rot < 0 || rot > h3::kHeadDim || rot % 16) return fail(H3B200_ERR_INVALID, "%s: rot_dim must be a multiple of 16, at most 128, got %lld", who, (long long)rot_dim);
+  if (freqs && freqs_dtype != H3B200_DTYPE_F32 && freqs_dtype != H3B200_DTYPE_BF16 && freqs_dtype != H3B200_DTYPE_F16)
+    return fail(H3B200_ERR_INVALID, "%s: freqs dtype code must be 0 (float32), 1 (float16) or 2 (bfloat16), got %d", who, freqs_dtype);
+  if ((slots_dtype | positions_dtype) & ~1) return fail(H3B200_ERR_INVALID, "%s: slots and positions are int64 (1) or int32 (0)", who);
+  if (freqs && !positions && freqs_rows < tokens) return fail(H3B200_ERR_INVALID, "%s: %lld rotation rows for %lld tokens without positions", who, (long long)freqs_rows, (long long)tokens);
+  if (tokens == 0) return H3B200_OK;
+  if (!k || !v || !k_cache || !v_cache || !slots || (q && !q_out)) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  h3::AppendKvArgs a;
+  a.q = q; a.k = k; a.v = v;
+  a.xs_t[0] = q_st; a.xs_t[1] = k_st; a.xs_t[2] = v_st;
+  a.xs_h[0] = q_sh; a.xs_h[1] = k_sh; a.xs_h[2] = v_sh;
+  a.q_out = q_out; a.qo_t = qo_st; a.qo_h = qo_sh;
+  a.cache[0] = k_cache; a.c_page[0] = kc_sp; a.c_head[0] = kc_sh; a.c_row[0] = kc_sr;
+  a.cache[1] = v_cache; a.c_page[1] = vc_sp; a.c_head[1] = vc_sh; a.c_row[1] = vc_sr;
+  a.pages = pages; a.page_size = page_size;
+  a.slot_of = slots; a.slot64 = slots_dtype;
+  a.position_of = positions; a.position64 = positions_dtype;
+  a.table = freqs; a.table_rows = freqs_rows; a.table_stride = f_st;
+  a.table_dtype = freqs_dtype == H3B200_DTYPE_F32 ? 0 : (freqs_dtype == H3B200_DTYPE_BF16 ? 1 : 2);
+  a.w[0] = q_weight; a.w[1] = k_weight;
+  a.tokens = tokens; a.heads = q ? heads : 0; a.kv_heads = kv_heads; a.rot = rot; a.eps = eps;
+  a.f16 = dtype == H3B200_DTYPE_F16;
+  return from_cuda(h3::launch_append_paged_kv(a, S(stream)), who);
+}
+
+int64_t h3b200_paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t table_width,
+                                            int64_t page_size) {
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || table_width < 0 || page_size <= 0) return 0;
+  return h3::paged_decode_workspace_bytes(batch, heads, kv_heads, table_width * page_size, current_sms());
+}
+
+int h3b200_paged_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, const void* k_cache, int64_t kc_sp,
+                                  int64_t kc_sh, int64_t kc_sr, const void* v_cache, int64_t vc_sp, int64_t vc_sh,
+                                  int64_t vc_sr, int64_t pages, int64_t page_size, const int32_t* page_table,
+                                  int64_t pt_sb, int64_t table_width, const int32_t* lengths, void* out, int64_t o_sb,
+                                  int64_t o_sh, float* lse, int64_t l_sb, int64_t l_sh, int64_t batch, int64_t heads,
+                                  int64_t kv_heads, float scale, int dtype, void* workspace, int64_t workspace_bytes,
+                                  h3b200_stream_t stream) {
+  H3_GUARD("paged_decode_attention", stream);
+  const char* who = "paged_decode_attention";
+  if (const int rc = attn_dtype(dtype, who)) return rc;
+  if (const int rc = paged_shape(pages, page_size, who)) return rc;
+  if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
+  if (batch < 0 || table_width < 0 || table_width > 0x7FFFFF00 / page_size) return fail(H3B200_ERR_INVALID, "%s: bad shape (a sequence holds fewer than 2^31 keys)", who);
+  if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(H3B200_ERR_INVALID, "%s: scale must be positive and finite", who);
+  if (batch == 0) return H3B200_OK;
+  if (!q || !out || !lengths || (table_width > 0 && (!page_table || (pages > 0 && (!k_cache || !v_cache))))) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  const int64_t need = h3b200_paged_decode_workspace_bytes(batch, heads, kv_heads, table_width, page_size);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
+  h3::PagedDecodeArgs a;
+  a.q = q; a.q_b = q_sb; a.q_h = q_sh;
+  a.k = k_cache; a.k_page = kc_sp; a.k_head = kc_sh; a.k_row = kc_sr;
+  a.v = v_cache; a.v_page = vc_sp; a.v_head = vc_sh; a.v_row = vc_sr;
+  a.table = page_table; a.t_b = pt_sb; a.t_h = 0; a.width = table_width;
+  a.pages = pages; a.page_size = page_size; a.rows = pages * page_size;
+  a.lengths = lengths;
+  a.out = out; a.o_b = o_sb; a.o_h = o_sh; a.lse = lse; a.l_b = l_sb; a.l_h = l_sh;
+  a.batch = batch; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale;
+  a.workspace = workspace; a.f16 = dtype == H3B200_DTYPE_F16;
+  return from_cuda(h3::launch_paged_decode(a, S(stream)), who);
+}
+
+int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t x_sh, int64_t tokens, int64_t heads,
+                                 int64_t block, int dtype, float* means, h3b200_stream_t stream) {
+  H3_GUARD("attention_block_means", stream);
+  const char* who = "attention_block_means";
+  if (const int rc = attn_dtype(dtype, who)) return rc;
+  if (tokens < 0 || heads < 0 || block <= 0 || block > (1 << 20)) return fail(H3B200_ERR_INVALID, "%s: bad shape", who);
+  if (tokens == 0 || heads == 0) return H3B200_OK;
+  if (!x || !means) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  return from_cuda(h3::launch_block_means(x, x_st, x_sh, tokens, heads, block, dtype == H3B200_DTYPE_F16, means, S(stream)), who);
+}
+
+int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t heads, int64_t kv_heads,
+                             int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal, int32_t* blocks,
+                             h3b200_stream_t stream) {
+  H3_GUARD("select_key_blocks", stream);
+  const char* who = "select_key_blocks";
+  if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
+  if (queries < 0 || keys < 0 || block <= 0 || block > (1 << 20) || top_k <= 0 || top_k > (1 << 24)) return fail(H3B200_ERR_INVALID, "%s: bad shape (top_k and block must be positive)", who);
+  if (queries == 0) return H3B200_OK;
+  const int64_t k_blocks = (keys + block - 1) / block;
+  if (k_blocks > h3::select_blocks_max()) return fail(H3B200_ERR_UNSUPPORTED, "%s: %lld key blocks, at most %lld are built", who, (long long)k_blocks, (long long)h3::select_blocks_max());
+  if (!q_means || (keys > 0 && !k_means) || !blocks) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  h3::SelectBlocksArgs a;
+  a.q_means = q_means; a.k_means = k_means; a.heads = heads; a.kv_heads = kv_heads;
+  a.q_blocks = (queries + h3::kQueryBlock - 1) / h3::kQueryBlock;
+  a.k_blocks = k_blocks; a.top_k = top_k; a.block = block; a.queries = queries; a.keys = keys;
+  a.causal = causal != 0; a.out = blocks;
+  return from_cuda(h3::launch_select_blocks(a, S(stream)), who);
+}
+
+int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k,
+                                            int64_t block) {
+  if (queries != 1 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || top_k <= 0 || block <= 0) return 0;
+  return h3::paged_decode_workspace_bytes(1, heads, kv_heads, top_k * block, current_sms());
+}
+
+int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks,
+                                  int64_t top_k, int64_t block, void* out, int64_t o_st, int64_t o_sh, float* lse,
+                                  int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys, int64_t heads,
+                                  int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
+                                  int64_t workspace_bytes, h3b200_stream_t stream) {
+  H3_GUARD("block_sparse_attention", stream);
+  const char* who = "block_sparse_attention";
+  if (const int rc = attn_dtype(dtype, who)) return rc;
+  if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
+  if (queries < 0 || keys <= 0 || top_k <= 0) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys and top_k must be positive)", who);
+  if (block != 64 && block != 128) return fail(H3B200_ERR_UNSUPPORTED, "%s: blocks of 64 or 128 keys are built, got %lld", who, (long long)block);
+  if (top_k > 0x7FFFFF00 / block) return fail(H3B200_ERR_INVALID, "%s: top_k too large", who);
+  if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(H3B200_ERR_INVALID, "%s: scale must be positive and finite", who);
+  if (queries == 0) return H3B200_OK;
+  if (!q || !k || !v || !blocks || !out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  if (queries == 1) {
+    // one token sees every key it lists (its position is the last one): the split kernel
+    // with the list as each head's page table
+    const int64_t need = h3b200_block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+      return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
+    h3::PagedDecodeArgs a;
+    a.q = q; a.q_b = 0; a.q_h = q_sh;
+    a.k = k; a.k_page = block * k_st; a.k_head = k_sh; a.k_row = k_st;
+    a.v = v; a.v_page = block * v_st; a.v_head = v_sh; a.v_row = v_st;
+    a.table = blocks; a.t_b = 0; a.t_h = top_k; a.width = top_k;
+    a.pages = (keys + block - 1) / block; a.page_size = block; a.rows = keys;
+    a.out = out; a.o_b = 0; a.o_h = o_sh; a.lse = lse; a.l_b = 0; a.l_h = l_sh;
+    a.batch = 1; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale;
+    a.workspace = workspace; a.f16 = dtype == H3B200_DTYPE_F16;
+    return from_cuda(h3::launch_paged_decode(a, S(stream)), who);
+  }
+  h3::SparseAttnArgs a;
+  a.q = q; a.k = k; a.v = v;
+  a.q_t = q_st; a.q_h = q_sh; a.k_t = k_st; a.k_h = k_sh; a.v_t = v_st; a.v_h = v_sh;
+  a.blocks = blocks;
+  a.queries = queries; a.keys = keys; a.heads = heads; a.kv_heads = kv_heads; a.top_k = top_k; a.block = block;
+  a.scale = scale; a.causal = causal != 0;
+  a.out = out; a.o_t = o_st; a.o_h = o_sh; a.lse = lse; a.l_t = l_st; a.l_h = l_sh;
+  a.f16 = dtype == H3B200_DTYPE_F16;
+  return from_cuda(h3::launch_block_sparse_attention(a, S(stream)), who);
+}
+
+}  // extern "C"

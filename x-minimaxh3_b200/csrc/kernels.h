@@ -278,6 +278,95 @@ cudaError_t launch_rms_adaln(const RmsAdalnArgs& a, cudaStream_t stream);
 cudaError_t launch_swiglu_rows(const void* x, int64_t ldx, void* y, int64_t ldy, int64_t m, int64_t k,
                                cudaStream_t stream);
 
+// ---------------------------------------------------------------------------
+// Attention after the Q/K/V build: 16-bit elements (bf16, or fp16 with f16), head dim
+// 128, element strides, 16-byte aligned rows. cudaErrorNotSupported outside that.
+// ---------------------------------------------------------------------------
+
+// Keys and values (and rotated queries) of new tokens into a paged cache (paged_kv.cu).
+// cache[i] (0 K, 1 V): page / head / row strides; slot = page * page_size + row, slots
+// outside the pool are skipped. table rows [rot / 2, 2, 2] at table_stride elements,
+// dtype 0 fp32, 1 bf16, 2 fp16; position_of null: row = token. w[i] (0 Q, 1 K): norm
+// weights or null.
+struct AppendKvArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  int64_t xs_t[3] = {0, 0, 0}, xs_h[3] = {0, 0, 0};
+  void* q_out = nullptr;
+  int64_t qo_t = 0, qo_h = 0;
+  void* cache[2] = {nullptr, nullptr};
+  int64_t c_page[2] = {0, 0}, c_head[2] = {0, 0}, c_row[2] = {0, 0};
+  int64_t pages = 0, page_size = 0;
+  const void* slot_of = nullptr;
+  const void* position_of = nullptr;
+  int slot64 = 1, position64 = 1;
+  const void* table = nullptr;
+  int table_dtype = 0;
+  int64_t table_rows = 0, table_stride = 0;
+  const void* w[2] = {nullptr, nullptr};
+  int64_t tokens = 0, heads = 0, kv_heads = 0, rot = 0;
+  float eps = 1e-6f;
+  bool f16 = false;
+};
+cudaError_t launch_append_paged_kv(const AppendKvArgs& a, cudaStream_t stream);
+
+// Attention of one token per sequence over pages (paged_attention.cu). table[b, h, i]
+// (strides t_b, t_h, 1; width entries) names the pages of sequence b and key head h; ids
+// outside [0, pages) hold no keys. rows: rows of the pool (the last page may end early).
+// lengths null: width * page_size keys. lse may be null.
+struct PagedDecodeArgs {
+  const void* q = nullptr;
+  int64_t q_b = 0, q_h = 0;
+  const void* k = nullptr;
+  int64_t k_page = 0, k_head = 0, k_row = 0;
+  const void* v = nullptr;
+  int64_t v_page = 0, v_head = 0, v_row = 0;
+  const int32_t* table = nullptr;
+  int64_t t_b = 0, t_h = 0, width = 0;
+  int64_t pages = 0, page_size = 0, rows = 0;
+  const int32_t* lengths = nullptr;
+  void* out = nullptr;
+  int64_t o_b = 0, o_h = 0;
+  float* lse = nullptr;
+  int64_t l_b = 0, l_h = 0;
+  int64_t batch = 0, heads = 0, kv_heads = 0;
+  float scale = 0.0f;
+  void* workspace = nullptr;  // paged_decode_workspace_bytes, 16-byte aligned
+  bool f16 = false;
+};
+int64_t paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms);
+cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream);
+
+constexpr int kQueryBlock = 128;  // query rows that share a selection of key blocks
+
+// fp32 [heads, ceil(tokens / block), 128] means of the blocks of x [tokens, heads, 128] (block_select.cu)
+cudaError_t launch_block_means(const void* x, int64_t x_t, int64_t x_h, int64_t tokens, int64_t heads, int64_t block,
+                               bool f16, float* means, cudaStream_t stream);
+// out [kv_heads, q_blocks, top_k]: selected key blocks, ascending, -1 behind them
+struct SelectBlocksArgs {
+  const float *q_means = nullptr, *k_means = nullptr;
+  int64_t heads = 0, kv_heads = 0, q_blocks = 0, k_blocks = 0, top_k = 0, block = 0, queries = 0, keys = 0;
+  bool causal = false;
+  int32_t* out = nullptr;
+};
+int64_t select_blocks_max();  // key blocks the kernel can score
+cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream);
+
+// Attention of 128-row query blocks over listed key blocks (sparse_attention.cu)
+struct SparseAttnArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;
+  int64_t q_t = 0, q_h = 0, k_t = 0, k_h = 0, v_t = 0, v_h = 0;
+  const int32_t* blocks = nullptr;  // [kv_heads, q_blocks, top_k]
+  int64_t queries = 0, keys = 0, heads = 0, kv_heads = 0, top_k = 0, block = 0;
+  float scale = 0.0f;
+  bool causal = false;
+  void* out = nullptr;
+  int64_t o_t = 0, o_h = 0;
+  float* lse = nullptr;
+  int64_t l_t = 0, l_h = 0;
+  bool f16 = false;
+};
+cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t stream);
+
 // 2-D tiled TMA descriptor (no interleave, 256-byte L2 promotion, no OOB fill);
 // false when the driver's encoder is unavailable or rejects the layout.
 bool encode_tmap_2d(CUtensorMap* map, CUtensorMapDataType dtype, const void* base, uint64_t inner, uint64_t rows,

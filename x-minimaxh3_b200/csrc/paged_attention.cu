@@ -1,0 +1,383 @@
+// Attention of one new token per sequence over a paged key / value cache.
+//
+//   s_j = scale q . k_j,  out = sum_j exp(s_j - m) v_j / l,  l = sum_j exp(s_j - m),  lse = m + ln l
+//
+// over the keys j < length of the sequence; key j is row j % page_size of page
+// table[j / page_size]. A sequence without keys gives 0 and lse = -inf.
+//
+// Bound: HBM. Every key and value row is read once for the whole group of query
+// heads that share it, 4 bytes per two multiply-adds and head, so the kernel
+// only has to keep enough loads in flight. One warp takes 16 keys at a time and
+// reads them straight into matrix-instruction operands; nothing is staged in
+// shared memory:
+//  * S^T = K Q^T (16 keys x 8 query heads, m16n8k16). The contraction index can
+//    be permuted freely, so lane (g, t) reads 16 contiguous bytes of key g (dims
+//    32 c + 8 t .. + 7) and uses them as two operand registers of two
+//    instructions; Q is held in the same order.
+//  * exp(S^T), rounded to 16 bits (the tensor core's operand type; the sum l
+//    takes the unrounded values), is transposed in registers (movmatrix).
+//  * O^T += V^T P^T: lane (g, t) reads 16 contiguous bytes (dims 8 g .. + 7) of
+//    keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs the keys with byte permutes. The
+//    output rows are permuted accordingly; each lane ends with 8 consecutive dims.
+// The small M of this work (the group's 1 to 16 heads) would leave a tcgen05
+// tile of 128 rows almost empty, and staging through shared memory for it would
+// cost what the direct loads save.
+//
+// Few sequences: the length is split over CTAs. Each split writes its
+// unnormalised O, its m and l; a second kernel joins them in the order of the
+// splits (no atomics: the same inputs always give the same bits).
+#include <algorithm>
+
+#include "attn_math.cuh"
+#include "kernels.h"
+
+namespace h3 {
+namespace {
+
+constexpr int kDecWarps = 4;
+constexpr int kDecThreads = kDecWarps * 32;
+
+struct DecodeParams {
+  const uint16_t* q;
+  int64_t q_b, q_h;
+  const uint16_t* k;
+  int64_t k_page, k_head, k_row;
+  const uint16_t* v;
+  int64_t v_page, v_head, v_row;
+  const int32_t* table;
+  int64_t t_b, t_h;
+  int64_t pages, rows;  // pages of the pool; rows < pages * page_size: the last page is not full
+  int width, page_size;
+  const int32_t* lengths;
+  uint16_t* out;
+  int64_t o_b, o_h;
+  float* lse;
+  int64_t l_b, l_h;
+  int heads, kv_heads, group, row_tiles;
+  float scale, scale_log2;
+  int splits, part_min;
+  float* ws_acc;
+  float2* ws_ml;
+};
+
+// Keys [begin, end) of split `s` of a sequence of `length` keys: even parts of at least
+// part_min keys, in whole 16-key steps. Returns the number of parts that hold keys.
+__device__ __forceinline__ int split_range(int length, int splits, int part_min, int s, int& begin, int& end) {
+  const int n = max(1, min(splits, (length + part_min - 1) / part_min));
+  const int per = max(16, ((length + n - 1) / n + 15) / 16 * 16);
+  begin = min(length, s * per);
+  end = min(length, begin + per);
+  return max(1, (length + per - 1) / per);
+}
+
+__device__ __forceinline__ int sequence_length(const DecodeParams& p, int b) {
+  const int cap = p.width * p.page_size;
+  return p.lengths == nullptr ? cap : max(0, min(cap, __ldg(p.lengths + b)));
+}
+
+template <bool F16, int NT>
+__global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_kernel(const DecodeParams p) {
+  using E = Elem16<F16>;
+  constexpr int R = 8 * NT;
+  __shared__ float sm_acc[kDecWarps][R][kHeadDim];
+  __shared__ float sm_m[kDecWarps][R], sm_l[kDecWarps][R];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int64_t item = blockIdx.x / p.splits;
+  const int split = (int)(blockIdx.x - item * p.splits);
+  const int rt = (int)(item % p.row_tiles);
+  const int kvh = (int)((item / p.row_tiles) % p.kv_heads);
+  const int b = (int)(item / ((int64_t)p.row_tiles * p.kv_heads));
+  const int length = sequence_length(p, b);
+  int begin, end;
+  const int parts = split_range(length, p.splits, p.part_min, split, begin, end);
+  if (split >= parts) return;
+  const int row0 = rt * R, rows = min(R, p.group - row0), head0 = kvh * p.group + row0;
+
+  uint32_t qf[NT][16];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (n * 8 + g < rows) w = ldg_v4(p.q + b * p.q_b + (head0 + n * 8 + g) * p.q_h + c * 32 + t * 8);
+      qf[n][4 * c] = w.x; qf[n][4 * c + 1] = w.y; qf[n][4 * c + 2] = w.z; qf[n][4 * c + 3] = w.w;
+    }
+  float acc[NT][8][4];
+  float m[NT][2], l[NT][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.0f;
+  }
+  const int32_t* table = p.table + b * p.t_b + kvh * p.t_h;
+  const uint16_t* kb = p.k + kvh * p.k_head;
+  const uint16_t* vb = p.v + kvh * p.v_head;
+
+  // page ids of the two 8-key halves of a step (page sizes are multiples of 8), -1: no keys
+  auto lookup = [&](int j) { return j < end ? __ldg(table + j / p.page_size) : -1; };
+  int id0 = lookup(begin + warp * 16), id1 = lookup(begin + warp * 16 + 8);
+  for (int j = begin + warp * 16; j < end; j += kDecWarps * 16) {
+    const int pid[2] = {id0, id1};
+    id0 = lookup(j + kDecWarps * 16);
+    id1 = lookup(j + kDecWarps * 16 + 8);
+    int valid[2];       // keys of each half that exist
+    int off[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int jj = j + 8 * h;
+      off[h] = jj % p.page_size;
+      valid[h] = min(8, end - jj);
+      if (pid[h] < 0 || pid[h] >= p.pages)
+        valid[h] = 0;  // no page of this pool: nothing is read
+      else
+        valid[h] = (int)min((int64_t)valid[h], p.rows - ((int64_t)pid[h] * p.page_size + off[h]));
+    }
+    uint4 kr[2][4], vr[2][2][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        kr[h][c] = make_uint4(0u, 0u, 0u, 0u);
+        if (g < valid[h]) kr[h][c] = ldg_stream_v4(kb + pid[h] * p.k_page + (off[h] + g) * p.k_row + c * 32 + t * 8);
+      }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          // keys that do not exist count as zero rows: 0 * (what lies there) could be NaN
+          vr[h][e][d] = make_uint4(0u, 0u, 0u, 0u);
+          if (2 * t + e < valid[h])
+            vr[h][e][d] = ldg_stream_v4(vb + pid[h] * p.v_page + (off[h] + 2 * t + e) * p.v_row + d * 64 + g * 8);
+        }
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        E::mma(s, kr[0][c].x, kr[1][c].x, kr[0][c].y, kr[1][c].y, qf[n][4 * c], qf[n][4 * c + 1]);
+        E::mma(s, kr[0][c].z, kr[1][c].z, kr[0][c].w, kr[1][c].w, qf[n][4 * c + 2], qf[n][4 * c + 3]);
+      }
+      if (g >= valid[0]) s[0] = s[1] = -INFINITY;
+      if (g >= valid[1]) s[2] = s[3] = -INFINITY;
+      float f[2], sub[2];
+      bool grew = false;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(s[e], s[2 + e]);
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+        const float mn = fmaxf(m[n][e], mx);
+        sub[e] = mn == -INFINITY ? 0.0f : mn * p.scale_log2;
+        f[e] = exp2f(m[n][e] * p.scale_log2 - sub[e]);  // exp2(-inf) = 0 before the first key
+        grew = grew || mn > m[n][e];
+        m[n][e] = mn;
+      }
+      if (__any_sync(0xFFFFFFFFu, grew)) {
+        l[n][0] *= f[0];
+        l[n][1] *= f[1];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          acc[n][i][0] *= f[0];
+          acc[n][i][1] *= f[1];
+          acc[n][i][2] *= f[0];
+          acc[n][i][3] *= f[1];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e] = exp2f(fmaf(s[e], p.scale_log2, -sub[e & 1]));
+        l[n][e & 1] += s[e];
+      }
+      pb[n][0] = movmatrix_trans(E::pack(s[0], s[1]));
+      pb[n][1] = movmatrix_trans(E::pack(s[2], s[3]));
+    }
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+      const uint32_t a[4] = {vr[0][0][d].x, vr[0][0][d].y, vr[0][0][d].z, vr[0][0][d].w};
+      const uint32_t c[4] = {vr[0][1][d].x, vr[0][1][d].y, vr[0][1][d].z, vr[0][1][d].w};
+      const uint32_t x[4] = {vr[1][0][d].x, vr[1][0][d].y, vr[1][0][d].z, vr[1][0][d].w};
+      const uint32_t y[4] = {vr[1][1][d].x, vr[1][1][d].y, vr[1][1][d].z, vr[1][1][d].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a0 = __byte_perm(a[i], c[i], 0x5410), a1 = __byte_perm(a[i], c[i], 0x7632);
+        const uint32_t a2 = __byte_perm(x[i], y[i], 0x5410), a3 = __byte_perm(x[i], y[i], 0x7632);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) E::mma(acc[n][d * 4 + i], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      }
+    }
+  }
+  // join the warps: lane (g, t) holds dims 64 d + 8 g + 2 i + {0, 1} of queries 2 t, 2 t + 1
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float s = l[n][e];
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, 4);
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, 8);
+      s += __shfl_xor_sync(0xFFFFFFFFu, s, 16);
+      const int r = n * 8 + 2 * t + e;
+      if (g == 0) {
+        sm_m[warp][r] = m[n][e];
+        sm_l[warp][r] = s;
+      }
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 o = make_float4(acc[n][d * 4 + 2 * h][e], acc[n][d * 4 + 2 * h][2 + e],
+                                       acc[n][d * 4 + 2 * h + 1][e], acc[n][d * 4 + 2 * h + 1][2 + e]);
+          *reinterpret_cast<float4*>(&sm_acc[warp][r][d * 64 + g * 8 + 4 * h]) = o;
+        }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * (kHeadDim / 4); i += kDecThreads) {
+    const int r = i / (kHeadDim / 4), d = (i % (kHeadDim / 4)) * 4;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) mx = fmaxf(mx, sm_m[w][r]);
+    float sum = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      const float f = mx == -INFINITY ? 0.0f : exp2f((sm_m[w][r] - mx) * p.scale_log2);
+      const float4 a = *reinterpret_cast<const float4*>(&sm_acc[w][r][d]);
+      sum = fmaf(sm_l[w][r], f, sum);
+      o.x = fmaf(a.x, f, o.x);
+      o.y = fmaf(a.y, f, o.y);
+      o.z = fmaf(a.z, f, o.z);
+      o.w = fmaf(a.w, f, o.w);
+    }
+    if (p.splits > 1) {
+      const int64_t at = (item * p.splits + split) * R + r;
+      *reinterpret_cast<float4*>(p.ws_acc + at * kHeadDim + d) = o;
+      if (d == 0) p.ws_ml[at] = make_float2(mx, sum);
+    } else {
+      const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);  // NaN stays
+      uint2 y;
+      y.x = E::pack(o.x * inv, o.y * inv);
+      y.y = E::pack(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(p.out + b * p.o_b + (head0 + r) * p.o_h + d) = y;
+      if (d == 0 && p.lse != nullptr)
+        p.lse[b * p.l_b + (head0 + r) * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum));
+    }
+  }
+}
+
+// One warp per (sequence, head): out = sum_s exp(m_s - m) O_s / sum_s exp(m_s - m) l_s.
+template <bool F16>
+__global__ void __launch_bounds__(128) decode_join_kernel(const DecodeParams p, int64_t total, int row_tile) {
+  using E = Elem16<F16>;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= total) return;
+  const int lane = threadIdx.x & 31;
+  const int b = (int)(row / p.heads), head = (int)(row % p.heads);
+  const int kvh = head / p.group, in_group = head % p.group;
+  const int64_t item = ((int64_t)b * p.kv_heads + kvh) * p.row_tiles + in_group / row_tile;
+  const int r = in_group % row_tile;
+  int begin, end;
+  const int parts = split_range(sequence_length(p, b), p.splits, p.part_min, 0, begin, end);
+  const int64_t at = item * p.splits * row_tile + r;
+  float mx = -INFINITY;
+  for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, __ldcg(&p.ws_ml[at + (int64_t)s * row_tile].x));
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, i));
+  float sum = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = __ldcg(&p.ws_ml[at + (int64_t)s * row_tile]);
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (at + (int64_t)s * row_tile) * kHeadDim) + lane);
+    const float f = mx == -INFINITY ? 0.0f : exp2f((ml.x - mx) * p.scale_log2);
+    sum = fmaf(ml.y, f, sum);
+    o.x = fmaf(a.x, f, o.x);
+    o.y = fmaf(a.y, f, o.y);
+    o.z = fmaf(a.z, f, o.z);
+    o.w = fmaf(a.w, f, o.w);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+  uint2 y;
+  y.x = E::pack(o.x * inv, o.y * inv);
+  y.y = E::pack(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(p.out + b * p.o_b + head * p.o_h + lane * 4) = y;
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[b * p.l_b + head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum));
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr int kPartMin = 64;     // keys: one 16-key step of each warp
+constexpr int kMaxSplits = 256;
+
+int row_tile_of(int64_t group) { return group <= 8 ? 8 : 16; }
+
+}  // namespace
+
+int paged_decode_splits(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms) {
+  const int64_t group = heads / kv_heads;
+  const int64_t items = batch * kv_heads * ((group + row_tile_of(group) - 1) / row_tile_of(group));
+  const int64_t most = std::max<int64_t>(1, (max_keys + kPartMin - 1) / kPartMin);
+  const int64_t want = (4ll * sms + items - 1) / items;
+  return (int)std::min<int64_t>(kMaxSplits, std::min(most, want));
+}
+
+int64_t paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms) {
+  const int64_t splits = paged_decode_splits(batch, heads, kv_heads, max_keys, sms);
+  if (splits == 1) return 0;
+  const int64_t group = heads / kv_heads, tile = row_tile_of(group);
+  const int64_t rows = batch * kv_heads * ((group + tile - 1) / tile) * splits * tile;
+  return rows * (kHeadDim * 4 + 8);
+}
+
+cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream) {
+  if (a.batch <= 0) return cudaSuccess;
+  DecodeParams p;
+  if (!aligned(a.q) || a.q_b % 8 || a.q_h % 8 || !aligned(a.k) || a.k_page % 8 || a.k_head % 8 || a.k_row % 8 ||
+      !aligned(a.v) || a.v_page % 8 || a.v_head % 8 || a.v_row % 8 || !aligned(a.out) || a.o_b % 8 || a.o_h % 8)
+    return cudaErrorNotSupported;
+  p.q = static_cast<const uint16_t*>(a.q); p.q_b = a.q_b; p.q_h = a.q_h;
+  p.k = static_cast<const uint16_t*>(a.k); p.k_page = a.k_page; p.k_head = a.k_head; p.k_row = a.k_row;
+  p.v = static_cast<const uint16_t*>(a.v); p.v_page = a.v_page; p.v_head = a.v_head; p.v_row = a.v_row;
+  p.table = a.table; p.t_b = a.t_b; p.t_h = a.t_h;
+  p.pages = a.pages; p.rows = a.rows; p.width = (int)a.width; p.page_size = (int)a.page_size;
+  p.lengths = a.lengths;
+  p.out = static_cast<uint16_t*>(a.out); p.o_b = a.o_b; p.o_h = a.o_h;
+  p.lse = a.lse; p.l_b = a.l_b; p.l_h = a.l_h;
+  p.heads = (int)a.heads; p.kv_heads = (int)a.kv_heads; p.group = (int)(a.heads / a.kv_heads);
+  const int tile = row_tile_of(p.group);
+  p.row_tiles = (p.group + tile - 1) / tile;
+  p.scale = a.scale;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  p.splits = paged_decode_splits(a.batch, a.heads, a.kv_heads, a.width * a.page_size, num_sms(dev));
+  p.part_min = kPartMin;
+  const int64_t items = a.batch * a.kv_heads * p.row_tiles;
+  if (items * p.splits > 0x7FFFFFFF) return cudaErrorNotSupported;
+  p.ws_acc = static_cast<float*>(a.workspace);
+  p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + items * p.splits * tile * kHeadDim);
+  const unsigned grid = (unsigned)(items * p.splits);
+  if (a.f16) {
+    if (tile == 8) paged_decode_kernel<true, 1><<<grid, kDecThreads, 0, stream>>>(p);
+    else paged_decode_kernel<true, 2><<<grid, kDecThreads, 0, stream>>>(p);
+  } else {
+    if (tile == 8) paged_decode_kernel<false, 1><<<grid, kDecThreads, 0, stream>>>(p);
+    else paged_decode_kernel<false, 2><<<grid, kDecThreads, 0, stream>>>(p);
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || p.splits == 1) return e;
+  const int64_t total = a.batch * a.heads;
+  const unsigned jgrid = (unsigned)((total + 3) / 4);
+  if (a.f16) decode_join_kernel<true><<<jgrid, 128, 0, stream>>>(p, total, tile);
+  else decode_join_kernel<false><<<jgrid, 128, 0, stream>>>(p, total, tile);
+  return cudaGetLastError();
+}
+
+}  // namespace h3

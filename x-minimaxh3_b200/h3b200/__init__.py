@@ -5,11 +5,21 @@ Public operators mirror the comfy_kitchen backend surface that
 ``quantize_int8_rowwise``, ``int8_linear_prequantized``, ``mm_int8``,
 ``w4a8_int8_linear``, ``rms_rope_split_half(_)``) plus the fused entry points
 ``fused_gated_mlp`` and ``adaln_rms_rope(_)``, and ``fused_gated_mlp_host`` for
-token buffers in host memory (copies overlapped with the MLP). All of them run hand-written CUDA
+token buffers in host memory (copies overlapped with the MLP). The attention that follows
+the Q/K/V build is here too: ``append_paged_kv`` with ``paged_decode_attention``, and
+``sparse_attention``. All of them run hand-written CUDA
 from ``libh3b200.so`` through its C ABI; there is no other backend.
 """
 
 from . import _lib
+from .attention import (  # noqa: F401
+    append_paged_kv,
+    attention_block_means,
+    block_sparse_attention,
+    paged_decode_attention,
+    select_key_blocks,
+    sparse_attention,
+)
 from .ops import (  # noqa: F401
     adaln_rms_rope,
     apply_input_act,

@@ -693,7 +693,8 @@ H3B200_API int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t
 
 /*
  * Key blocks that block-sparse attention reads, from block means of queries (blocks of
- * 128) and keys (blocks of `block`):
+ * 128) and keys (blocks of `block`; k_means rows at head / block strides in elements,
+ * multiples of 4, 16-byte aligned; q_means contiguous):
  *   score[i, j] = sum over the heads h of the group of q_means[h, i] . k_means[kv_head, j]  (64 bits)
  * blocks[kv_head, i]: the top_k highest scores' j in ascending order (equal scores: the
  * lowest j; NaN below every number), -1 behind them when fewer blocks can be seen.
@@ -701,9 +702,9 @@ H3B200_API int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t
  * behind the query block's last position are never selected; those that hold a
  * position at or behind its first one come before all others.
  */
-H3B200_API int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t heads, int64_t kv_heads,
-                                        int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
-                                        int32_t* blocks, h3b200_stream_t stream);
+H3B200_API int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb,
+                                        int64_t heads, int64_t kv_heads, int64_t queries, int64_t keys, int64_t block,
+                                        int64_t top_k, int causal, int32_t* blocks, h3b200_stream_t stream);
 
 /*
  * Attention of query blocks of 128 rows over listed key blocks:
@@ -725,6 +726,23 @@ H3B200_API int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_
                                              int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
                                              float scale, int causal, int dtype, void* workspace,
                                              int64_t workspace_bytes, h3b200_stream_t stream);
+
+/*
+ * h3b200_attention_block_means of Q (and of K where k_means is NULL),
+ * h3b200_select_key_blocks into `blocks` (int32 [kv_heads, ceil(queries / 128), top_k]) and
+ * h3b200_block_sparse_attention over them, in one call; arguments as there.
+ * workspace: h3b200_sparse_attention_workspace_bytes bytes, 256-byte aligned.
+ */
+H3B200_API int64_t h3b200_sparse_attention_workspace_bytes(int64_t queries, int64_t keys, int64_t heads,
+                                                           int64_t kv_heads, int64_t top_k, int64_t block,
+                                                           int has_k_means);
+H3B200_API int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                       int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const float* k_means,
+                                       int64_t km_sh, int64_t km_sb, int64_t top_k, int64_t block, int32_t* blocks,
+                                       void* out, int64_t o_st, int64_t o_sh, float* lse, int64_t l_st, int64_t l_sh,
+                                       int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads, float scale,
+                                       int causal, int dtype, void* workspace, int64_t workspace_bytes,
+                                       h3b200_stream_t stream);
 
 #ifdef __cplusplus
 }

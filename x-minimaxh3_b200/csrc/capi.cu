@@ -1529,9 +1529,9 @@ int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t x_sh, int6
   return from_cuda(h3::launch_block_means(x, x_st, x_sh, tokens, heads, block, dtype == H3B200_DTYPE_F16, means, S(stream)), who);
 }
 
-int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t heads, int64_t kv_heads,
-                             int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal, int32_t* blocks,
-                             h3b200_stream_t stream) {
+int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb, int64_t heads,
+                             int64_t kv_heads, int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
+                             int32_t* blocks, h3b200_stream_t stream) {
   H3_GUARD("select_key_blocks", stream);
   const char* who = "select_key_blocks";
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
@@ -1541,7 +1541,7 @@ int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t
   if (k_blocks > h3::select_blocks_max()) return fail(H3B200_ERR_UNSUPPORTED, "%s: %lld key blocks, at most %lld are built", who, (long long)k_blocks, (long long)h3::select_blocks_max());
   if (!q_means || (keys > 0 && !k_means) || !blocks) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
   h3::SelectBlocksArgs a;
-  a.q_means = q_means; a.k_means = k_means; a.heads = heads; a.kv_heads = kv_heads;
+  a.q_means = q_means; a.k_means = k_means; a.km_h = km_sh; a.km_b = km_sb; a.heads = heads; a.kv_heads = kv_heads;
   a.q_blocks = (queries + h3::kQueryBlock - 1) / h3::kQueryBlock;
   a.k_blocks = k_blocks; a.top_k = top_k; a.block = block; a.queries = queries; a.keys = keys;
   a.causal = causal != 0; a.out = blocks;
@@ -1596,6 +1596,45 @@ int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, con
   a.out = out; a.o_t = o_st; a.o_h = o_sh; a.lse = lse; a.l_t = l_st; a.l_h = l_sh;
   a.f16 = dtype == H3B200_DTYPE_F16;
   return from_cuda(h3::launch_block_sparse_attention(a, S(stream)), who);
+}
+
+int64_t h3b200_sparse_attention_workspace_bytes(int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
+                                                int64_t top_k, int64_t block, int has_k_means) {
+  if (queries <= 0 || keys <= 0 || heads <= 0 || kv_heads <= 0 || block <= 0) return 0;
+  const int64_t row = h3::kHeadDim * 4;
+  return round_up(heads * ((queries + h3::kQueryBlock - 1) / h3::kQueryBlock) * row, 256) +
+         (has_k_means ? 0 : round_up(kv_heads * ((keys + block - 1) / block) * row, 256)) +
+         h3b200_block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block);
+}
+
+int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                            const void* v, int64_t v_st, int64_t v_sh, const float* k_means, int64_t km_sh,
+                            int64_t km_sb, int64_t top_k, int64_t block, int32_t* blocks, void* out, int64_t o_st,
+                            int64_t o_sh, float* lse, int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys,
+                            int64_t heads, int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
+                            int64_t workspace_bytes, h3b200_stream_t stream) {
+  H3_GUARD("sparse_attention", stream);
+  const char* who = "sparse_attention";
+  if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
+  if (queries < 0 || keys <= 0 || top_k <= 0 || block <= 0 || block > (1 << 20)) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys, top_k and block must be positive)", who);
+  if (queries == 0) return H3B200_OK;
+  const int64_t need = h3b200_sparse_attention_workspace_bytes(queries, keys, heads, kv_heads, top_k, block, k_means != nullptr);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
+  const int64_t row = h3::kHeadDim * 4, k_blocks = (keys + block - 1) / block;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  float* qm = reinterpret_cast<float*>(base);
+  base += round_up(heads * ((queries + h3::kQueryBlock - 1) / h3::kQueryBlock) * row, 256);
+  if (const int rc = h3b200_attention_block_means(q, q_st, q_sh, queries, heads, h3::kQueryBlock, dtype, qm, stream)) return rc;
+  if (k_means == nullptr) {
+    float* km = reinterpret_cast<float*>(base);
+    base += round_up(kv_heads * k_blocks * row, 256);
+    if (const int rc = h3b200_attention_block_means(k, k_st, k_sh, keys, kv_heads, block, dtype, km, stream)) return rc;
+    k_means = km; km_sh = k_blocks * h3::kHeadDim; km_sb = h3::kHeadDim;
+  }
+  if (const int rc = h3b200_select_key_blocks(qm, k_means, km_sh, km_sb, heads, kv_heads, queries, keys, block, top_k, causal, blocks, stream)) return rc;
+  return h3b200_block_sparse_attention(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
+                                       heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, stream);
 }
 
 }  // extern "C"

@@ -343,7 +343,8 @@ cudaError_t launch_block_means(const void* x, int64_t x_t, int64_t x_h, int64_t 
                                bool f16, float* means, cudaStream_t stream);
 // out [kv_heads, q_blocks, top_k]: selected key blocks, ascending, -1 behind them
 struct SelectBlocksArgs {
-  const float *q_means = nullptr, *k_means = nullptr;
+  const float *q_means = nullptr, *k_means = nullptr;  // q contiguous, k rows at strides
+  int64_t km_h = 0, km_b = 0;
   int64_t heads = 0, kv_heads = 0, q_blocks = 0, k_blocks = 0, top_k = 0, block = 0, queries = 0, keys = 0;
   bool causal = false;
   int32_t* out = nullptr;

@@ -78,9 +78,77 @@ __device__ __forceinline__ void load_coef(const void* table, int dtype, int64_t 
   other = second ? a : b;
 }
 
+// Rows [lo, hi) of the token's Q or K heads: y = rstd (A x + B x_partner) with the norm
+// weights folded into the rotation coefficients A, B once per run.
+template <bool F16>
+__device__ __forceinline__ void turn_rows(const uint16_t* src, int64_t src_h, uint16_t* dst,
+                                          int64_t dst_h, int lo, int hi, const uint16_t* w, float eps, bool rotated,
+                                          int partner, const float (&ca)[8], const float (&cb)[8]) {
+  using E = Elem16<F16>;
+  const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15;
+  uint64_t a2[4], b2[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float a0 = ca[2 * i], a1 = ca[2 * i + 1], b0 = cb[2 * i], b1 = cb[2 * i + 1];
+    if (w != nullptr) {
+      const uint32_t wo = __ldg(reinterpret_cast<const uint32_t*>(w + l * 8) + i);
+      const uint32_t wp = __ldg(reinterpret_cast<const uint32_t*>(w + partner * 8) + i);
+      a0 *= E::lo(wo);
+      a1 *= E::hi(wo);
+      b0 *= E::lo(wp);
+      b1 *= E::hi(wp);
+    }
+    a2[i] = f2_pack(a0, a1);
+    b2[i] = f2_pack(b0, b1);
+  }
+  for (int r0 = lo; r0 < hi; r0 += 2 * kAppendUnroll) {
+    uint4 x[kAppendUnroll];
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
+      const int r = r0 + 2 * u + half;
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < hi) x[u] = ldg_v4(src + r * src_h);
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
+      if (r0 + 2 * u >= hi) break;  // warp-uniform: the shuffles below see both halves
+      const int r = r0 + 2 * u + half;
+      uint32_t own[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      uint64_t f[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t other = __shfl_sync(0xFFFFFFFFu, own[i], partner, 16);
+        if (!rotated) other = 0u;  // B is 0 there; 0 * inf must not be
+        f[i] = f2_pack(E::lo(own[i]), E::hi(own[i]));
+        y[i] = f2_fma(a2[i], f[i], f2_mul(b2[i], f2_pack(E::lo(other), E::hi(other))));
+      }
+      if (w != nullptr) {
+        uint64_t s = 0ull;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = f2_fma(f[i], f[i], s);
+        float s0, s1;
+        f2_unpack(s, s0, s1);
+        s0 += s1;
+#pragma unroll
+        for (int i = 8; i > 0; i >>= 1) s0 += __shfl_xor_sync(0xFFFFFFFFu, s0, i, 16);
+        const float rstd = rsqrtf(s0 * (1.0f / kHeadDim) + eps);
+        const uint64_t rr = f2_pack(rstd, rstd);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = f2_mul(y[i], rr);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float a, b;
+        f2_unpack(y[i], a, b);
+        own[i] = E::pack(a, b);
+      }
+      if (r < hi) stg_v4(dst + r * dst_h, make_uint4(own[0], own[1], own[2], own[3]));
+    }
+  }
+}
+
 template <bool F16>
 __global__ void __launch_bounds__(kAppendThreads) append_paged_kv_kernel(const AppendParams p) {
-  using E = Elem16<F16>;
   const int64_t warp = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const int64_t token = warp / p.chunks;
   if (token >= p.tokens) return;
@@ -88,92 +156,49 @@ __global__ void __launch_bounds__(kAppendThreads) append_paged_kv_kernel(const A
   const int64_t slot = load_index(p.slot_of, p.slot64, token);
   if (slot < 0 || slot >= p.slots) return;  // padding: nothing of this token is written
   const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15;
-  const int nq = p.q_out != nullptr ? p.heads : 0;
-  const int rows = nq + 2 * p.kv_heads;
-  const int begin = chunk * p.rows_per_warp, end = min(rows, begin + p.rows_per_warp);
-  if (begin >= end) return;
+  const int nq = p.q_out != nullptr ? p.heads : 0, nk = nq + p.kv_heads;
+  const int begin = chunk * p.rows_per_warp, end = min(nk + p.kv_heads, begin + p.rows_per_warp);
 
-  const int step = p.rot >> 4;  // lanes of half the rotated dims
-  const bool rotated = l < 2 * step;
-  const int second = l >= step ? 1 : 0;
-  const int partner = rotated ? (second ? l - step : l + step) : l;
-  float ca[8], cb[8];
-  if (rotated && begin < nq + p.kv_heads) {
-    const int64_t row = p.position_of == nullptr ? token : load_index(p.position_of, p.position64, token);
-    const bool known = row >= 0 && row < p.table_rows;
+  const int64_t page = slot / p.page_size, row_in_page = slot - page * p.page_size;
+  if (begin < nk) {
+    const int step = p.rot >> 4;  // lanes of half the rotated dims
+    const bool rotated = l < 2 * step;
+    const int second = l >= step ? 1 : 0;
+    const int partner = rotated ? (second ? l - step : l + step) : l;
+    float ca[8], cb[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      ca[i] = cb[i] = __int_as_float(0x7FC00000);  // a position outside the table: NaN, not a wrong rotation
-      if (known) load_coef(p.table, p.table_dtype, row * p.table_stride, (l - second * step) * 8 + i, second, ca[i], cb[i]);
+      ca[i] = 1.0f;
+      cb[i] = 0.0f;
     }
+    if (rotated) {
+      const int64_t row = p.position_of == nullptr ? token : load_index(p.position_of, p.position64, token);
+      const bool known = row >= 0 && row < p.table_rows;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ca[i] = cb[i] = __int_as_float(0x7FC00000);  // a position outside the table: NaN, not a wrong rotation
+        if (known) load_coef(p.table, p.table_dtype, row * p.table_stride, (l - second * step) * 8 + i, second, ca[i], cb[i]);
+      }
+    }
+    if (begin < nq)
+      turn_rows<F16>(p.x[0] + token * p.xs_t[0] + l * 8, p.xs_h[0], p.q_out + token * p.qo_t + l * 8, p.qo_h, begin,
+                     min(end, nq), p.w[0], p.eps, rotated, partner, ca, cb);
+    if (end > nq)
+      turn_rows<F16>(p.x[1] + token * p.xs_t[1] + l * 8, p.xs_h[1],
+                     p.cache[0] + page * p.c_page[0] + row_in_page * p.c_row[0] + l * 8, p.c_head[0],
+                     max(begin, nq) - nq, min(end, nk) - nq, p.w[1], p.eps, rotated, partner, ca, cb);
   }
-  const int64_t page = slot / p.page_size, row_in_page = slot - page * p.page_size;
-
-  for (int r0 = begin; r0 < end; r0 += 2 * kAppendUnroll) {
-    uint4 x[kAppendUnroll];
+  if (end > nk) {
+    const uint16_t* src = p.x[2] + token * p.xs_t[2] + l * 8;
+    uint16_t* dst = p.cache[1] + page * p.c_page[1] + row_in_page * p.c_row[1] + l * 8;
+    for (int r0 = max(begin, nk) - nk; r0 < end - nk; r0 += 4 * kAppendUnroll) {
+      uint4 x[2 * kAppendUnroll];
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
-      const int r = r0 + 2 * u + half;
-      x[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < end) {
-        const int which = r < nq ? 0 : (r < nq + p.kv_heads ? 1 : 2);
-        const int head = which == 0 ? r : r - nq - (which - 1) * p.kv_heads;
-        x[u] = ldg_v4(p.x[which] + token * p.xs_t[which] + head * p.xs_h[which] + l * 8);
-      }
-    }
+      for (int u = 0; u < 2 * kAppendUnroll; ++u)
+        if (r0 + 2 * u + half < end - nk) x[u] = ldg_v4(src + (r0 + 2 * u + half) * p.xs_h[2]);
 #pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
-      const int r = r0 + 2 * u + half;
-      if (r0 + 2 * u >= end) break;  // warp-uniform: the shuffles below see both halves
-      const int which = r < nq ? 0 : (r < nq + p.kv_heads ? 1 : 2);
-      const int head = which == 0 ? r : r - nq - (which - 1) * p.kv_heads;
-      uint32_t own[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, other[4];
-      float f[8], g[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        other[i] = __shfl_sync(0xFFFFFFFFu, own[i], partner, 16);
-        f[2 * i] = E::lo(own[i]);
-        f[2 * i + 1] = E::hi(own[i]);
-      }
-      const uint16_t* w = which < 2 ? p.w[which] : nullptr;
-      float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
-#pragma unroll
-      for (int i = 8; i > 0; i >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, i, 16);
-      if (r >= end) continue;
-      if (which < 2) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          g[2 * i] = E::lo(other[i]);
-          g[2 * i + 1] = E::hi(other[i]);
-        }
-        if (w != nullptr) {
-          const float rstd = rsqrtf(ss * (1.0f / kHeadDim) + p.eps);
-          const uint4 wo = __ldg(reinterpret_cast<const uint4*>(w + l * 8));
-          const uint4 wp = __ldg(reinterpret_cast<const uint4*>(w + partner * 8));
-          const uint32_t wow[4] = {wo.x, wo.y, wo.z, wo.w}, wpw[4] = {wp.x, wp.y, wp.z, wp.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            f[2 * i] *= rstd * E::lo(wow[i]);
-            f[2 * i + 1] *= rstd * E::hi(wow[i]);
-            g[2 * i] *= rstd * E::lo(wpw[i]);
-            g[2 * i + 1] *= rstd * E::hi(wpw[i]);
-          }
-        }
-        if (rotated) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = fmaf(ca[i], f[i], cb[i] * g[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) own[i] = E::pack(f[2 * i], f[2 * i + 1]);
-      }
-      uint16_t* y;
-      if (which == 0)
-        y = p.q_out + token * p.qo_t + head * p.qo_h;
-      else
-        y = p.cache[which - 1] + page * p.c_page[which - 1] + head * p.c_head[which - 1] + row_in_page * p.c_row[which - 1];
-      stg_v4(y + l * 8, make_uint4(own[0], own[1], own[2], own[3]));
+      for (int u = 0; u < 2 * kAppendUnroll; ++u)
+        if (r0 + 2 * u + half < end - nk) stg_v4(dst + (r0 + 2 * u + half) * p.c_head[1], x[u]);
     }
   }
 }

@@ -34,11 +34,7 @@ bool encode_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t d0, uint64
 
 namespace {
 
-// 2 x 4 softmax warps, then one warpgroup whose first two warps are the TMA and the MMA
-// warp. A softmax thread holds a row of 128 scores, so its warpgroups take registers
-// from the third: 2 x 208 + 80 <= 3 x 168 per thread triple at launch.
-constexpr int kSpThreads = 384;
-constexpr int kSoftRegs = 208, kCtrlRegs = 80;
+constexpr int kSpThreads = 320;    // 2 x 4 softmax warps, TMA warp, MMA warp
 constexpr int kSubKeys = 64;  // keys of one TMA box; a tile holds two
 constexpr int kTileBytes = 128 * kHeadDim * 2;     // 32 KB: a Q, K or V tile
 constexpr int kHalfBytes = kTileBytes / 2;         // dims 0..63 or 64..127 of 128 rows
@@ -112,6 +108,23 @@ __device__ __forceinline__ int sub_key(const SparseParams& p, const int32_t* lis
   return id * p.block + (sub - e * per) * kSubKeys;
 }
 
+// 32 lanes x 16 columns, as tmem_ld32 / tmem_st32
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
 struct Stream {
   int64_t item;
   int head, q_block;
@@ -138,8 +151,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t* kv_full = q_full + 2;                                  // [kRing]
   uint64_t* kv_empty = kv_full + kRing;                            // [kRing]
   uint64_t* s_full = kv_empty + kRing;                             // [2] scores are in TMEM
-  uint64_t* p_full = s_full + 2;                                   // [2] P is in TMEM, O is rescaled
-  uint64_t* o_full = p_full + 2;                                   // [2] O is complete
+  uint64_t* p_full = s_full + 2;                                   // [2][2] a half of P is in TMEM, O is rescaled
+  uint64_t* o_full = p_full + 4;                                   // [2] O is complete
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
   int* tiles_of = reinterpret_cast<int*>(tmem_slot + 1);           // [2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -148,7 +161,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);  // one arrival per softmax warp
+      mbar_init(&p_full[2 * i], 4);  // one arrival per softmax warp
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
     }
     for (int i = 0; i < kRing; ++i) {
@@ -186,10 +200,6 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const int n0 = tiles_of[0], n1 = tiles_of[1];
   const int nmax = max(n0, n1);
-  if (warp < 8)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-  else
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
 
   if (warp == 8) {
     if (lane == 0) {
@@ -260,14 +270,19 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         for (int s = 0; s < 2 && ok; ++s) {
           if (i >= n[s]) continue;
           const int slot = used % kRing;
-          ok = mbar_wait(&kv_full[slot], (used / kRing) & 1, kErrSpMma) && mbar_wait(&p_full[s], i & 1, kErrSpMma);
-          if (!ok) break;
-          tc_fence_after();
+          ok = mbar_wait(&kv_full[slot], (used / kRing) & 1, kErrSpMma);
           const uint32_t b = smem_u32(smem + kOffRing + slot * kTileBytes);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, umma_desc_mn_sw128(b + k * 16 * 128), kIdescO,
-                        i > 0 || k > 0 ? 1u : 0u);
+          for (int h = 0; h < 2; ++h) {  // the first half's product runs while the second half's P is computed
+            ok = ok && mbar_wait(&p_full[2 * s + h], i & 1, kErrSpMma);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)
+              umma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, umma_desc_mn_sw128(b + k * 16 * 128), kIdescO,
+                          i > 0 || k > 0 ? 1u : 0u);
+          }
+          if (!ok) break;
           umma_commit(&kv_empty[slot]);
           ++used;
           if (i + 1 < n[s])
@@ -276,7 +291,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
             umma_commit(&o_full[s]);
         }
     }
-  } else if (warp < 8) {
+  } else {
     // ---------------- softmax: thread = row ----------------
     const int s = warp >> 2;
     const int n = s ? n1 : n0;
@@ -317,9 +332,10 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       float mx[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(x[c][0]);
+        mx[c] = fmaxf(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]));
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(x[c][e]));
+        for (int e = 2; e < 32; e += 2)  // two at a time: one three-input maximum
+          mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(x[c][e])), __uint_as_float(x[c][e + 1]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool grow = (top - m) * p.scale_log2 > kRescaleLog2;  // also the first finite score (m = -inf)
@@ -330,41 +346,43 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         if (grow) m = top;
         l *= f;
         // the product of the tile before is complete: its commit came before s_full's
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_o + c * 32, o);
+#pragma unroll 1
+        for (int c = 0; c < 8; ++c) {
+          uint32_t o[16];
+          tmem_ld16(t_o + c * 16, o);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st32(t_o + c * 32, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st16(t_o + c * 16, o);
         }
       }
       const float sub = m == -INFINITY ? 0.0f : m * p.scale_log2;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(-sub, -sub);
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float y = ex2_approx(fmaf(__uint_as_float(x[c][e]), p.scale_log2, -sub));
-          sum[e & 3] += y;
-          x[c][e] = __float_as_uint(y);
+        for (int e = 0; e < 16; ++e) {
+          float a, b;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), scale2, sub2), a, b);
+          a = ex2_approx(a);
+          b = ex2_approx(b);
+          sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, b));
+          w[e] = E::pack(a, b);
         }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const int j = c * 64 + 2 * e;
-          w[e] = E::pack(__uint_as_float(x[j >> 5][j & 31]), __uint_as_float(x[j >> 5][(j & 31) + 1]));
+        tmem_st16(t_s + c * 16, w);  // over columns already read
+        if (c & 1) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * s + (c >> 1)]);
         }
-        tmem_st32(t_s + c * 32, w);
       }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[s]);
+      float s0, s1, s2, s3;
+      f2_unpack(sum[0], s0, s1);
+      f2_unpack(sum[1], s2, s3);
+      l += (s0 + s1) + (s2 + s3);
     }
     if (st.item < p.items && s < p.streams && ok) {
       if (n > 0) ok = mbar_wait(&o_full[s], 0, kErrSpOut);

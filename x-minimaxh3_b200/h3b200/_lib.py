@@ -92,11 +92,15 @@ SIGNATURES = {
                                              _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _f32,
                                              _i32, _p, _i64, _p]),
     "h3b200_attention_block_means": (_i32, [_p, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p]),
-    "h3b200_select_key_blocks": (_i32, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p]),
+    "h3b200_select_key_blocks": (_i32, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _p, _p]),
     "h3b200_block_sparse_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64]),
     "h3b200_block_sparse_attention": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64,
                                              _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _p, _i64,
                                              _p]),
+    "h3b200_sparse_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i64, _i64, _i64, _i32]),
+    "h3b200_sparse_attention": (_i32, [_p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p,
+                                       _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _i32, _p,
+                                       _i64, _p]),
     "h3b200_tp_comm_create": (_i32, [_i32, _i32, _i64, _i64, _i64, _i64, ctypes.POINTER(_p), _p]),
     "h3b200_tp_comm_open": (_i32, [_p, _p]),
     "h3b200_tp_comm_link_local": (_i32, [ctypes.POINTER(_p), _i32]),

@@ -6,6 +6,9 @@ on the current stream of the tensors' device, ``ValueError`` for arguments outsi
 contract, ``NotImplementedError`` for valid ones that are not built, no fallback. Elements
 are bf16 or fp16 (one type for all tensors of a call), the head dim is 128. The operators
 are for inference: they record nothing for autograd.
+
+A call on one token is bound by the host, so each operator asks a tensor for its shape,
+strides and type once and makes one call into the library.
 """
 
 from __future__ import annotations
@@ -16,7 +19,7 @@ import math
 import torch
 
 from . import _lib
-from .ops import _TABLE_DTYPE_CODES, _need_cuda, _stream
+from .ops import _TABLE_DTYPE_CODES
 
 __all__ = [
     "append_paged_kv",
@@ -32,20 +35,27 @@ QUERY_BLOCK = 128   # query rows that share a selection of key blocks
 _DTYPES = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 _INDEX_CODES = {torch.int64: 1, torch.int32: 0}
 _SCALE = 1.0 / math.sqrt(HEAD_DIM)
+_current = contextlib.nullcontext()
 
 
-def _same_device(first: torch.Tensor, *ts):
-    _need_cuda(first, *ts)
+def _device(*ts) -> int:
+    """Index of the CUDA device that holds every given tensor."""
+    index = ts[0].get_device()
     for t in ts:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"all tensors must be on one device, got {first.device} and {t.device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in ts if t is not None]}")
+    if index < 0 or not ts[0].is_cuda:
+        raise ValueError("h3b200 operators take CUDA tensors only (no CPU fallback)")
+    return index
 
 
-def _on(t: torch.Tensor):
+def _on(index: int):
     """The tensors' device for the launch (nothing to do when it is the current one)."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+    return _current if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -55,35 +65,36 @@ def _dtype_code(t: torch.Tensor) -> int:
     return code
 
 
-def _thd(t: torch.Tensor, name: str, dtype: torch.dtype) -> torch.Tensor:
-    """[1, T, H, 128] / [T, H, 128] with unit stride on the head dim -> [T, H, 128] view."""
-    if t.dim() == 4:
-        if t.shape[0] != 1:
+def _thd(t: torch.Tensor, name: str, dtype: torch.dtype):
+    """(shape, strides) of [1, T, H, 128] / [T, H, 128] with unit stride on the head dim, as [T, H, 128]."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 4:
+        if shape[0] != 1:
             raise ValueError(f"{name}: batch dimension must be 1 (packed token layout)")
-        t = t[0]
-    if t.dim() != 3 or t.shape[2] != HEAD_DIM:
+        shape, stride = shape[1:], stride[1:]
+    if len(shape) != 3 or shape[2] != HEAD_DIM:
         raise ValueError(f"{name}: expected [T, H, {HEAD_DIM}] or [1, T, H, {HEAD_DIM}], got {tuple(t.shape)}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.stride(2) != 1:
+    if stride[2] != 1:
         raise ValueError(f"{name}: head_dim must have unit stride")
-    return t
+    return shape, stride
 
 
-def _cache(t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
-    if t.dim() != 4 or t.shape[3] != HEAD_DIM:
-        raise ValueError(f"{name}: expected [pages, kv_heads, page_size, {HEAD_DIM}], got {tuple(t.shape)}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.stride(3) != 1:
-        raise ValueError(f"{name}: head_dim must have unit stride")
-
-
-def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype) -> None:
-    _cache(k_cache, "k_cache", dtype)
-    _cache(v_cache, "v_cache", dtype)
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache {tuple(k_cache.shape)} and v_cache {tuple(v_cache.shape)} must have the same shape")
+def _caches(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype):
+    """(shape, K strides, V strides) of a paged cache."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4 or shape[3] != HEAD_DIM:
+        raise ValueError(f"k_cache: expected [pages, kv_heads, page_size, {HEAD_DIM}], got {tuple(shape)}")
+    if v_cache.shape != shape:
+        raise ValueError(f"k_cache {tuple(shape)} and v_cache {tuple(v_cache.shape)} must have the same shape")
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+        raise ValueError(f"k_cache and v_cache must be {dtype}, got {k_cache.dtype} and {v_cache.dtype}")
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError("k_cache and v_cache: head_dim must have unit stride")
+    if shape[2] == 0 or shape[2] % 8:
+        raise ValueError(f"page_size must be a positive multiple of 8, got {shape[2]}")
+    return shape, ks, vs
 
 
 def _groups(heads: int, kv_heads: int) -> None:
@@ -91,23 +102,29 @@ def _groups(heads: int, kv_heads: int) -> None:
         raise ValueError(f"query heads ({heads}) must be a positive multiple of key heads ({kv_heads})")
 
 
-def _weight(w: torch.Tensor | None, name: str, like: torch.Tensor) -> torch.Tensor | None:
-    if w is None:
-        return None
-    w = w.detach().to(device=like.device, dtype=like.dtype).reshape(-1).contiguous()
+def _weight(w: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    if w.dtype is not like.dtype or w.get_device() != like.get_device() or not w.is_contiguous():
+        w = w.detach().to(device=like.device, dtype=like.dtype).contiguous()
     if w.numel() != HEAD_DIM:
         raise ValueError(f"{name} must have {HEAD_DIM} elements")
     return w
 
 
-def _index(t: torch.Tensor | None, name: str, tokens: int) -> int:
-    if t is None:
-        return 1
+def _index(t: torch.Tensor, name: str, tokens: int) -> int:
     code = _INDEX_CODES.get(t.dtype)
-    if code is None or t.dim() != 1 or t.shape[0] != tokens or not t.is_contiguous():
+    if code is None or t.shape != (tokens,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int64 or int32 tensor of {tokens} elements (one per token), got "
                          f"{t.dtype} {tuple(t.shape)}")
     return code
+
+
+def _scale_of(scale) -> float:
+    if scale is None:
+        return _SCALE
+    scale = float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
 
 
 def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -119,10 +136,11 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
     ``k``, ``v`` [T, kv_heads, 128] (or [1, T, ...]; views of a packed projection work) go to
     row ``slots[t] % page_size`` of page ``slots[t] // page_size`` of ``k_cache`` / ``v_cache``
-    [pages, kv_heads, page_size, 128], in place (a cache kept as [pages, page_size, kv_heads,
-    128] is passed as its ``transpose(1, 2)``). A token whose slot is -1 (or any value outside
-    the pool) is padding: nothing of it is written, its ``q_out`` row included. The slots of
-    one call must differ; which token a slot named twice ends up with is not defined.
+    [pages, kv_heads, page_size, 128] (page_size a multiple of 8), in place (a cache kept as
+    [pages, page_size, kv_heads, 128] is passed as its ``transpose(1, 2)``). A token whose slot
+    is -1 (or any value outside the pool) is padding: nothing of it is written, its ``q_out``
+    row included. The slots of one call must differ; which token a slot named twice ends up
+    with is not defined.
 
     With ``k_weight`` [128], K gets per-head RMSNorm first; with ``frequencies`` [P, R / 2, 2,
     2] (or [1, P, 1, R / 2, 2, 2]; fp32, bf16 or fp16), split-half RoPE of its first R dims by
@@ -133,76 +151,73 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     Norm and rotation are fp32 and rounded once, at the store (:func:`h3b200.qknorm_rope_strided_`
     also rounds between the two, as the reference it reproduces does). Returns ``q_out``
     (None without ``q``)."""
-    _same_device(k, v, k_cache, v_cache, slots, frequencies, positions, q, q_out)
+    dtype = k.dtype
     code = _dtype_code(k)
-    k3, v3 = _thd(k, "k", k.dtype), _thd(v, "v", k.dtype)
-    if k3.shape != v3.shape:
-        raise ValueError(f"k {tuple(k3.shape)} and v {tuple(v3.shape)} must have the same shape")
-    t, kv_heads, _ = k3.shape
-    _caches(k_cache, v_cache, k.dtype)
-    if k_cache.shape[1] != kv_heads:
-        raise ValueError(f"the cache holds {k_cache.shape[1]} heads, k has {kv_heads}")
-    if kv_heads == 0:
-        raise ValueError("k and v need at least one head")
+    dev = _device(k, v, k_cache, v_cache, slots, frequencies, positions, q, q_out)
+    shape, ks = _thd(k, "k", dtype)
+    vshape, vs = _thd(v, "v", dtype)
+    t, kv_heads, _ = shape
+    if vshape != shape or kv_heads == 0:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(vshape)} must have the same shape, with at least one head")
+    cshape, kcs, vcs = _caches(k_cache, v_cache, dtype)
+    if cshape[1] != kv_heads:
+        raise ValueError(f"the cache holds {cshape[1]} heads, k has {kv_heads}")
     slot_code = _index(slots, "slots", t)
-    position_code = _index(positions, "positions", t)
-    rows = stride = rot = table_code = 0
-    f = frequencies
-    if f is not None:
-        if f.dim() == 6 and f.shape[0] == 1 and f.shape[2] == 1:
+    position_code, position_ptr = 1, None
+    freq_ptr, rows, stride, rot, table_code = None, 0, 0, 0, 0
+    if frequencies is not None:
+        f = frequencies
+        fshape = f.shape
+        if len(fshape) == 6 and fshape[0] == 1 and fshape[2] == 1:
             f = f[0, :, 0]
-        if f.dim() != 4 or f.shape[2] != 2 or f.shape[3] != 2:
+            fshape = f.shape
+        if len(fshape) != 4 or fshape[2] != 2 or fshape[3] != 2:
             raise ValueError(f"frequencies must be [P, R / 2, 2, 2] or [1, P, 1, R / 2, 2, 2], got "
                              f"{tuple(frequencies.shape)}")
-        if f.dtype not in _TABLE_DTYPE_CODES:
+        table_code = _TABLE_DTYPE_CODES.get(f.dtype)
+        if table_code is None:
             raise ValueError(f"frequencies must be float32, float16 or bfloat16, got {f.dtype}")
-        rot = 2 * f.shape[1]
+        rows, rot = fshape[0], 2 * fshape[1]
         if rot == 0 or rot > HEAD_DIM or rot % 16:
             raise ValueError(f"frequencies must rotate a multiple of 16 dims, at most {HEAD_DIM}, got {rot}")
-        if f.stride(3) != 1 or f.stride(2) != 2 or f.stride(1) != 4:
+        if not f.is_contiguous() and f.stride()[1:] != (4, 2, 1):
             f = f.contiguous()
-        rows, stride, table_code = f.shape[0], f.stride(0), _TABLE_DTYPE_CODES[f.dtype]
-        if positions is None and rows < t:
+        stride, freq_ptr = f.stride(0), f.data_ptr()
+        if positions is not None:
+            position_code, position_ptr = _index(positions, "positions", t), positions.data_ptr()
+        elif rows < t:
             raise ValueError(f"frequencies hold {rows} rows for {t} tokens; pass positions to pick rows")
     elif positions is not None:
         raise ValueError("positions need frequencies")
-    kw, qw = _weight(k_weight, "k_weight", k3), None
-    q3 = qo3 = None
+    kw = kw_ptr = qw = qw_ptr = q_ptr = qo_ptr = None
+    if k_weight is not None:
+        kw = _weight(k_weight, "k_weight", k)
+        kw_ptr = kw.data_ptr()
+    qs = qos = (0, 0)
     heads = 0
     if q is not None:
-        q3 = _thd(q, "q", k.dtype)
-        heads = q3.shape[1]
-        if q3.shape[0] != t or heads == 0:
-            raise ValueError(f"q must be [{t}, heads, {HEAD_DIM}], got {tuple(q3.shape)}")
-        qw = _weight(q_weight, "q_weight", q3)
+        qshape, qs = _thd(q, "q", dtype)
+        heads = qshape[1]
+        if qshape[0] != t or heads == 0:
+            raise ValueError(f"q must be [{t}, heads, {HEAD_DIM}], got {tuple(qshape)}")
+        if q_weight is not None:
+            qw = _weight(q_weight, "q_weight", q)
+            qw_ptr = qw.data_ptr()
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        qo3 = _thd(q_out, "q_out", k.dtype)
-        if qo3.shape != q3.shape:
+            q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        qoshape, qos = _thd(q_out, "q_out", dtype)
+        if qoshape != qshape:
             raise ValueError("q_out must have q's shape")
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_weight is not None or q_out is not None:
         raise ValueError("q_weight and q_out need q")
-    with _on(k3):
-        _lib.call("h3b200_append_paged_kv", None if q3 is None else q3.data_ptr(), 0 if q3 is None else q3.stride(0),
-                  0 if q3 is None else q3.stride(1), None if q3 is None else qo3.data_ptr(),
-                  0 if q3 is None else qo3.stride(0), 0 if q3 is None else qo3.stride(1),
-                  None if qw is None else qw.data_ptr(), k3.data_ptr(), k3.stride(0), k3.stride(1),
-                  None if kw is None else kw.data_ptr(), v3.data_ptr(), v3.stride(0), v3.stride(1),
-                  k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(),
-                  v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_cache.shape[0], k_cache.shape[2],
-                  slots.data_ptr(), slot_code, None if positions is None else positions.data_ptr(), position_code,
-                  None if f is None else f.data_ptr(), table_code, rows, stride, rot, float(eps), code, t, heads,
-                  kv_heads, _stream(k3))
+    with _on(dev):
+        _lib.call("h3b200_append_paged_kv", q_ptr, qs[0], qs[1], qo_ptr, qos[0], qos[1], qw_ptr, k.data_ptr(), ks[0],
+                  ks[1], kw_ptr, v.data_ptr(), vs[0], vs[1], k_cache.data_ptr(), kcs[0], kcs[1], kcs[2],
+                  v_cache.data_ptr(), vcs[0], vcs[1], vcs[2], cshape[0], cshape[2], slots.data_ptr(), slot_code,
+                  position_ptr, position_code, freq_ptr, table_code, rows, stride, rot, eps, code, t, heads, kv_heads,
+                  _stream(dev))
     return q_out
-
-
-def _scale_of(scale) -> float:
-    if scale is None:
-        return _SCALE
-    scale = float(scale)
-    if not 0.0 < scale < 1e30:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    return scale
 
 
 def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
@@ -221,39 +236,42 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     split over the GPU by its length at run time, so a captured graph stays valid while
     ``lengths`` and ``page_table`` change in place; the same inputs give the same bits.
     Returns ``out`` [B, heads, 128], with ``return_lse`` (out, fp32 [B, heads] log-sum-exp)."""
-    _same_device(q, k_cache, v_cache, page_table, lengths, out)
+    dtype = q.dtype
     code = _dtype_code(q)
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.stride(2) != 1:
-        raise ValueError(f"q must be [B, heads, {HEAD_DIM}] with unit stride on the head dim, got {tuple(q.shape)}")
-    b, heads, _ = q.shape
-    _caches(k_cache, v_cache, q.dtype)
-    pages, kv_heads, page_size, _ = k_cache.shape
+    dev = _device(q, k_cache, v_cache, page_table, lengths, out)
+    qshape, qs = q.shape, q.stride()
+    if len(qshape) != 3 or qshape[2] != HEAD_DIM or qs[2] != 1:
+        raise ValueError(f"q must be [B, heads, {HEAD_DIM}] with unit stride on the head dim, got {tuple(qshape)}")
+    b, heads, _ = qshape
+    (pages, kv_heads, page_size, _), ks, vs = _caches(k_cache, v_cache, dtype)
     _groups(heads, kv_heads)
-    if page_size == 0 or page_size % 8:
-        raise ValueError(f"page_size must be a positive multiple of 8, got {page_size}")
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != b or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    tshape, ts = page_table.shape, page_table.stride()
+    if page_table.dtype is not torch.int32 or len(tshape) != 2 or tshape[0] != b or (tshape[1] > 1 and ts[1] != 1):
         raise ValueError(f"page_table must be int32 [{b}, width] with unit stride, got {page_table.dtype} "
-                         f"{tuple(page_table.shape)}")
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (b,) or not lengths.is_contiguous():
+                         f"{tuple(tshape)}")
+    if lengths.dtype is not torch.int32 or lengths.shape != (b,) or not lengths.is_contiguous():
         raise ValueError(f"lengths must be a contiguous int32 tensor of {b} elements, got {lengths.dtype} "
                          f"{tuple(lengths.shape)}")
     scale = _scale_of(scale)
     if out is None:
-        out = torch.empty((b, heads, HEAD_DIM), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
-        raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} with unit stride on the head dim")
-    lse = torch.empty((b, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    width = page_table.shape[1]
-    with _on(q):
-        nbytes = int(_lib.load().h3b200_paged_decode_workspace_bytes(b, heads, kv_heads, width, page_size))
-        work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _lib.call("h3b200_paged_decode_attention", q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(),
-                  k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(), v_cache.stride(0),
-                  v_cache.stride(1), v_cache.stride(2), pages, page_size, page_table.data_ptr(), page_table.stride(0),
-                  width, lengths.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-                  None if lse is None else lse.data_ptr(), heads, 1, b, heads, kv_heads, scale, code,
-                  None if work is None else work.data_ptr(), nbytes, _stream(q))
+        out = torch.empty(qshape, dtype=dtype, device=q.device)
+    elif out.shape != qshape or out.dtype is not dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be {dtype} {tuple(qshape)} with unit stride on the head dim")
+    lse = lse_ptr = work = work_ptr = None
+    if return_lse:
+        lse = torch.empty((b, heads), dtype=torch.float32, device=q.device)
+        lse_ptr = lse.data_ptr()
+    width = tshape[1]
+    os = out.stride()
+    with _on(dev):
+        nbytes = _lib.load().h3b200_paged_decode_workspace_bytes(b, heads, kv_heads, width, page_size)
+        if nbytes:
+            work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            work_ptr = work.data_ptr()
+        _lib.call("h3b200_paged_decode_attention", q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], ks[2],
+                  v_cache.data_ptr(), vs[0], vs[1], vs[2], pages, page_size, page_table.data_ptr(), ts[0], width,
+                  lengths.data_ptr(), out.data_ptr(), os[0], os[1], lse_ptr, heads, 1, b, heads, kv_heads, scale, code,
+                  work_ptr, nbytes, _stream(dev))
     return (out, lse) if return_lse else out
 
 
@@ -263,25 +281,24 @@ def attention_block_means(x: torch.Tensor, block_size: int) -> torch.Tensor:
     Summed in 64 bits and rounded once: :func:`select_key_blocks` compares products of
     them. A program that keeps its keys keeps their means too, and passes them to
     :func:`sparse_attention` as ``k_means``."""
-    _need_cuda(x)
     code = _dtype_code(x)
-    x3 = _thd(x, "x", x.dtype)
+    dev = _device(x)
+    (t, h, _), xs = _thd(x, "x", x.dtype)
     block_size = int(block_size)
     if block_size <= 0 or block_size > 1 << 20:
         raise ValueError(f"block_size must be positive (at most 2^20), got {block_size}")
-    t, h, _ = x3.shape
     means = torch.empty((h, -(-t // block_size), HEAD_DIM), dtype=torch.float32, device=x.device)
-    with _on(x3):
-        _lib.call("h3b200_attention_block_means", x3.data_ptr(), x3.stride(0), x3.stride(1), t, h, block_size, code,
-                  means.data_ptr(), _stream(x3))
+    with _on(dev):
+        _lib.call("h3b200_attention_block_means", x.data_ptr(), xs[0], xs[1], t, h, block_size, code,
+                  means.data_ptr(), _stream(dev))
     return means
 
 
 def _means(t: torch.Tensor, name: str, heads: int | None, blocks: int) -> None:
-    if t.dtype != torch.float32 or t.dim() != 3 or t.shape[1:] != (blocks, HEAD_DIM) or not t.is_contiguous() or (
+    if t.dtype is not torch.float32 or t.dim() != 3 or t.shape[1:] != (blocks, HEAD_DIM) or t.stride(2) != 1 or (
             heads is not None and t.shape[0] != heads):
-        raise ValueError(f"{name} must be contiguous float32 [{heads or 'heads'}, {blocks}, {HEAD_DIM}], got {t.dtype} "
-                         f"{tuple(t.shape)}")
+        raise ValueError(f"{name} must be float32 [{heads or 'heads'}, {blocks}, {HEAD_DIM}] with unit stride on the "
+                         f"head dim, got {t.dtype} {tuple(t.shape)}")
 
 
 def select_key_blocks(q_means: torch.Tensor, k_means: torch.Tensor, top_k: int, queries: int, keys: int,
@@ -295,7 +312,7 @@ def select_key_blocks(q_means: torch.Tensor, k_means: torch.Tensor, top_k: int, 
 
     ``causal``: query row r stands at position ``r + keys - queries``. Blocks that start
     behind the query block are never selected, and those that reach into it come first."""
-    _same_device(q_means, k_means)
+    dev = _device(q_means, k_means)
     queries, keys, block_size, top_k = int(queries), int(keys), int(block_size), int(top_k)
     if queries < 0 or keys < 0 or block_size <= 0 or top_k <= 0:
         raise ValueError("top_k and block_size must be positive, queries and keys not negative")
@@ -304,23 +321,42 @@ def select_key_blocks(q_means: torch.Tensor, k_means: torch.Tensor, top_k: int, 
     _means(k_means, "k_means", None, kb)
     heads, kv_heads = q_means.shape[0], k_means.shape[0]
     _groups(heads, kv_heads)
+    q_means = q_means.contiguous()
     blocks = torch.empty((kv_heads, qb, top_k), dtype=torch.int32, device=q_means.device)
-    with _on(q_means):
-        _lib.call("h3b200_select_key_blocks", q_means.data_ptr(), k_means.data_ptr(), heads, kv_heads, queries, keys,
-                  block_size, top_k, int(bool(causal)), blocks.data_ptr(), _stream(q_means))
+    with _on(dev):
+        _lib.call("h3b200_select_key_blocks", q_means.data_ptr(), k_means.data_ptr(), k_means.stride(0),
+                  k_means.stride(1), heads, kv_heads, queries, keys, block_size, top_k, int(bool(causal)),
+                  blocks.data_ptr(), _stream(dev))
     return blocks
 
 
 def _qkv(q, k, v):
-    _same_device(q, k, v)
+    dtype = q.dtype
     code = _dtype_code(q)
-    q3, k3, v3 = _thd(q, "q", q.dtype), _thd(k, "k", q.dtype), _thd(v, "v", q.dtype)
-    if k3.shape != v3.shape:
-        raise ValueError(f"k {tuple(k3.shape)} and v {tuple(v3.shape)} must have the same shape")
-    _groups(q3.shape[1], k3.shape[1])
-    if k3.shape[0] == 0:
-        raise ValueError("k and v need at least one token")
-    return q3, k3, v3, code
+    qshape, qs = _thd(q, "q", dtype)
+    kshape, ks = _thd(k, "k", dtype)
+    vshape, vs = _thd(v, "v", dtype)
+    if kshape != vshape or kshape[0] == 0:
+        raise ValueError(f"k {tuple(kshape)} and v {tuple(vshape)} must have the same shape, with at least one token")
+    _groups(qshape[1], kshape[1])
+    return code, qshape, qs, kshape, ks, vs
+
+
+def _block_size(block_size) -> int:
+    block_size = int(block_size)
+    if block_size not in (64, 128):
+        raise NotImplementedError(f"key blocks of 64 or 128 keys are built, got {block_size}")
+    return block_size
+
+
+def _out(out, q, qshape):
+    """(out, its [T, H] strides)."""
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    oshape, os = _thd(out, "out", q.dtype)
+    if oshape != qshape:
+        raise ValueError("out must have q's shape")
+    return out, os
 
 
 def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, blocks: torch.Tensor,
@@ -336,33 +372,27 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bl
     zeros (and lse -inf). Under ``causal`` all values of a listed block must be finite: those
     a row may not see enter its products with weight zero.
     Returns ``out`` [T, heads, 128], with ``return_lse`` (out, fp32 [T, heads] log-sum-exp)."""
-    q3, k3, v3, code = _qkv(q, k, v)
-    _same_device(q3, blocks, out)
-    t, heads, _ = q3.shape
-    s, kv_heads, _ = k3.shape
-    block_size = int(block_size)
-    if block_size not in (64, 128):
-        raise NotImplementedError(f"key blocks of 64 or 128 keys are built, got {block_size}")
-    if blocks.dtype != torch.int32 or blocks.dim() != 3 or blocks.shape[:2] != (kv_heads, -(-t // QUERY_BLOCK)) or (
-            blocks.shape[2] == 0 or not blocks.is_contiguous()):
+    dev = _device(q, k, v, blocks, out)
+    code, qshape, qs, kshape, ks, vs = _qkv(q, k, v)
+    t, heads, _ = qshape
+    s, kv_heads, _ = kshape
+    block_size = _block_size(block_size)
+    bshape = blocks.shape
+    if blocks.dtype is not torch.int32 or len(bshape) != 3 or bshape[:2] != (kv_heads, -(-t // QUERY_BLOCK)) or (
+            bshape[2] == 0 or not blocks.is_contiguous()):
         raise ValueError(f"blocks must be contiguous int32 [{kv_heads}, {-(-t // QUERY_BLOCK)}, top_k], got "
-                         f"{blocks.dtype} {tuple(blocks.shape)}")
+                         f"{blocks.dtype} {tuple(bshape)}")
     scale = _scale_of(scale)
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    o3 = _thd(out, "out", q.dtype)
-    if o3.shape != q3.shape:
-        raise ValueError("out must have q's shape")
+    out, os = _out(out, q, qshape)
     lse = torch.empty((t, heads), dtype=torch.float32, device=q.device) if return_lse else None
-    top_k = blocks.shape[2]
-    with _on(q3):
-        nbytes = int(_lib.load().h3b200_block_sparse_workspace_bytes(t, heads, kv_heads, top_k, block_size))
+    top_k = bshape[2]
+    with _on(dev):
+        nbytes = _lib.load().h3b200_block_sparse_workspace_bytes(t, heads, kv_heads, top_k, block_size)
         work = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-        _lib.call("h3b200_block_sparse_attention", q3.data_ptr(), q3.stride(0), q3.stride(1), k3.data_ptr(),
-                  k3.stride(0), k3.stride(1), v3.data_ptr(), v3.stride(0), v3.stride(1), blocks.data_ptr(), top_k,
-                  block_size, o3.data_ptr(), o3.stride(0), o3.stride(1), None if lse is None else lse.data_ptr(),
-                  heads, 1, t, s, heads, kv_heads, scale, int(bool(causal)), code,
-                  None if work is None else work.data_ptr(), nbytes, _stream(q3))
+        _lib.call("h3b200_block_sparse_attention", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1],
+                  v.data_ptr(), vs[0], vs[1], blocks.data_ptr(), top_k, block_size, out.data_ptr(), os[0], os[1],
+                  None if lse is None else lse.data_ptr(), heads, 1, t, s, heads, kv_heads, scale, int(bool(causal)),
+                  code, None if work is None else work.data_ptr(), nbytes, _stream(dev))
     return (out, lse) if return_lse else out
 
 
@@ -377,21 +407,30 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: i
     means of its keys, as it does when it generates one token at a time. ``top_k`` of at
     least the number of key blocks is dense attention.
     Returns ``out``, or a tuple (out, lse, blocks) of what was asked for, in this order."""
-    q3, k3, v3, _ = _qkv(q, k, v)
-    top_k, block_size = int(top_k), int(block_size)
-    if block_size not in (64, 128):
-        raise NotImplementedError(f"key blocks of 64 or 128 keys are built, got {block_size}")
+    dev = _device(q, k, v, k_means, out)
+    code, qshape, qs, kshape, ks, vs = _qkv(q, k, v)
+    t, heads, _ = qshape
+    s, kv_heads, _ = kshape
+    top_k, block_size = int(top_k), _block_size(block_size)
     if top_k <= 0:
         raise ValueError(f"top_k must be positive, got {top_k}")
     scale = _scale_of(scale)
-    t, s = q3.shape[0], k3.shape[0]
-    if k_means is None:
-        k_means = attention_block_means(k3, block_size)
-    else:
-        _same_device(q3, k_means)
-        _means(k_means, "k_means", k3.shape[1], -(-s // block_size))
-    blocks = select_key_blocks(attention_block_means(q3, QUERY_BLOCK), k_means, top_k, t, s, block_size, causal)
-    r = block_sparse_attention(q, k3, v3, blocks, block_size, scale, causal, out, return_lse)
-    if not return_blocks:
-        return r
-    return (*r, blocks) if return_lse else (r, blocks)
+    km_ptr, kms = None, (0, 0)
+    if k_means is not None:
+        _means(k_means, "k_means", kv_heads, -(-s // block_size))
+        km_ptr, kms = k_means.data_ptr(), k_means.stride()
+    out, os = _out(out, q, qshape)
+    device = q.device
+    lse = torch.empty((t, heads), dtype=torch.float32, device=device) if return_lse else None
+    blocks = torch.empty((kv_heads, -(-t // QUERY_BLOCK), top_k), dtype=torch.int32, device=device)
+    with _on(dev):
+        nbytes = _lib.load().h3b200_sparse_attention_workspace_bytes(t, s, heads, kv_heads, top_k, block_size,
+                                                                     k_means is not None)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _lib.call("h3b200_sparse_attention", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                  vs[0], vs[1], km_ptr, kms[0], kms[1], top_k, block_size, blocks.data_ptr(), out.data_ptr(), os[0],
+                  os[1], None if lse is None else lse.data_ptr(), heads, 1, t, s, heads, kv_heads, scale,
+                  int(bool(causal)), code, work.data_ptr(), nbytes, _stream(dev))
+    if return_lse:
+        return (out, lse, blocks) if return_blocks else (out, lse)
+    return (out, blocks) if return_blocks else out

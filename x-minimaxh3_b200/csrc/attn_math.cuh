@@ -68,6 +68,13 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   return r;
 }
 
+// three-input maximum (sm_100); NaN operands are dropped, as by fmaxf
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // transpose of an 8 x 8 matrix of 16-bit values held one row per four lanes
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t w) {
   uint32_t r;

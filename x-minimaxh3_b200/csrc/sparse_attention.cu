@@ -34,7 +34,7 @@ bool encode_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t d0, uint64
 
 namespace {
 
-constexpr int kSpThreads = 320;    // 2 x 4 softmax warps, TMA warp, MMA warp
+constexpr int kSpThreads = 352;    // 2 x 4 softmax warps, TMA warp, one MMA warp per stream
 constexpr int kSubKeys = 64;  // keys of one TMA box; a tile holds two
 constexpr int kTileBytes = 128 * kHeadDim * 2;     // 32 KB: a Q, K or V tile
 constexpr int kHalfBytes = kTileBytes / 2;         // dims 0..63 or 64..127 of 128 rows
@@ -153,7 +153,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t* s_full = kv_empty + kRing;                             // [2] scores are in TMEM
   uint64_t* p_full = s_full + 2;                                   // [2][2] a half of P is in TMEM, O is rescaled
   uint64_t* o_full = p_full + 4;                                   // [2] O is complete
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t* turn = o_full + 2;                                     // [2] the stream's products of a tile are issued
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
   int* tiles_of = reinterpret_cast<int*>(tmem_slot + 1);           // [2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_init(&p_full[2 * i], 4);  // one arrival per softmax warp
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
+      mbar_init(&turn[i], 1);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -242,54 +244,71 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       for (int j = (issued > kRing ? issued - kRing : 0); j < issued; ++j)
         mbar_wait(&kv_full[j % kRing], (j / kRing) & 1, kErrSpDrain, 200000000ull);
     }
-  } else if (warp == 9) {
+  } else if (warp >= 9) {
     if (lane == 0) {
-      // ---------------- MMA issuer ----------------
+      // ---------------- MMA issuers: warp 9 + s serves stream s ----------------
+      // An issuing thread is held until its instruction enters the (short) tensor queue,
+      // so its waits for softmax and loads would leave the tensor core idle; with an
+      // issuer per stream they run beside the other stream's products. The issuers take
+      // turns (turn[s]: stream s has issued its i-th P V and next Q K^T): left to
+      // themselves they interleave instruction by instruction, both softmaxes then start
+      // together, and the exponentials of one no longer hide behind the products of the
+      // other (2,126 us on the 21 x 39 x 40 grid, 24 heads, 64 of 512 blocks). Ring slots
+      // keep the producer's order over both streams: an issuer counts past the other's tiles.
       constexpr uint32_t kIdescS = idesc_f16kind(F16, false), kIdescO = idesc_f16kind(F16, true);
-      int used = 0;
-      bool ok = true;
-      const int n[2] = {n0, n1};
-      auto scores = [&](int s) {
-        const int slot = used % kRing;
-        if (!mbar_wait(&kv_full[slot], (used / kRing) & 1, kErrSpMma)) return false;
-        tc_fence_after();
-        const uint32_t a = smem_u32(smem + s * kTileBytes), b = smem_u32(smem + kOffRing + slot * kTileBytes);
+      const int s = warp - 9, n = s ? n1 : n0, other = s ? n0 : n1;
+      const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
+      const uint64_t q_desc = umma_desc_sw128(smem_u32(smem + s * kTileBytes));
+      const uint32_t ring = smem_u32(smem + kOffRing);
+      int at = s == 1 && other > 0 ? 1 : 0;  // ring position of this stream's next tile
+      auto scores = [&]() {
+        const int slot = at % kRing;
+        const uint64_t k_desc = umma_desc_sw128(ring + slot * kTileBytes);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-          umma_bf16(tmem + s * 128, umma_desc_sw128(a + off), umma_desc_sw128(b + off), kIdescS, k > 0 ? 1u : 0u);
+          const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
+          umma_bf16(t_s, q_desc + off, k_desc + off, kIdescS, k > 0 ? 1u : 0u);
         }
-        umma_commit(&kv_empty[slot]);
         umma_commit(&s_full[s]);
-        ++used;
-        return true;
+        umma_commit(&kv_empty[slot]);
       };
-      for (int s = 0; s < 2 && ok; ++s)
-        if (n[s] > 0) ok = mbar_wait(&q_full[s], 0, kErrSpMma) && scores(s);
-      for (int i = 0; i < nmax && ok; ++i)
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (i >= n[s]) continue;
-          const int slot = used % kRing;
-          ok = mbar_wait(&kv_full[slot], (used / kRing) & 1, kErrSpMma);
-          const uint32_t b = smem_u32(smem + kOffRing + slot * kTileBytes);
+      bool ok = n > 0 && mbar_wait(&q_full[s], 0, kErrSpMma) &&
+                mbar_wait(&kv_full[at % kRing], (at / kRing) & 1, kErrSpMma);
+      if (ok) {
+        tc_fence_after();
+        scores();
+      }
+      at = (n0 > 0 ? 1 : 0) + (n1 > 0 ? 1 : 0) + (s == 1 ? (other > 0 ? 1 : 0) + (other > 1 ? 1 : 0) : 0);
+      for (int i = 0; i < n && ok; ++i) {
+        const int slot = at % kRing;
+        ok = mbar_wait(&kv_full[slot], (at / kRing) & 1, kErrSpMma);
+        if (i + 1 < n) ok = ok && mbar_wait(&kv_full[(at + 1) % kRing], ((at + 1) / kRing) & 1, kErrSpMma);
+        ok = ok && mbar_wait(&p_full[2 * s], i & 1, kErrSpMma);
+        const int before = s == 0 ? i - 1 : i;  // the other stream's tile whose turn comes first
+        if (before >= 0 && before < other) ok = ok && mbar_wait(&turn[1 - s], before & 1, kErrSpMma);
+        const uint64_t v_desc = umma_desc_mn_sw128(ring + slot * kTileBytes);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {  // the first half's product runs while the second half's P is computed
-            ok = ok && mbar_wait(&p_full[2 * s + h], i & 1, kErrSpMma);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; ++k)
-              umma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, umma_desc_mn_sw128(b + k * 16 * 128), kIdescO,
-                          i > 0 || k > 0 ? 1u : 0u);
-          }
+        for (int h = 0; h < 2; ++h) {  // the first half's product runs while the second half's P is computed
+          if (h == 1) ok = ok && mbar_wait(&p_full[2 * s + 1], i & 1, kErrSpMma);
           if (!ok) break;
-          umma_commit(&kv_empty[slot]);
-          ++used;
-          if (i + 1 < n[s])
-            ok = scores(s);  // executes after the product above, which reads the columns it overwrites
-          else
-            umma_commit(&o_full[s]);
+          tc_fence_after();
+#pragma unroll
+          for (int k = 4 * h; k < 4 * h + 4; ++k)
+            umma_f16_ts(t_o, t_s + k * 8, v_desc + ((k * 16 * 128) >> 4), kIdescO, i > 0 || k > 0 ? 1u : 0u);
         }
+        if (!ok) break;
+        if (i + 1 < n) {
+          ++at;
+          scores();  // executes after the product above, which reads the columns it overwrites
+          // then the other stream's V and next K: tile i of stream 1, tile i + 1 of stream 0
+          const int j = s == 0 ? i : i + 1;
+          at += 1 + (j < other ? 1 : 0) + (j + 1 < other ? 1 : 0);
+        } else {
+          umma_commit(&o_full[s]);
+        }
+        mbar_arrive(&turn[s]);
+        umma_commit(&kv_empty[slot]);
+      }
     }
   } else {
     // ---------------- softmax: thread = row ----------------
@@ -334,8 +353,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       for (int c = 0; c < 4; ++c) {
         mx[c] = fmaxf(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]));
 #pragma unroll
-        for (int e = 2; e < 32; e += 2)  // two at a time: one three-input maximum
-          mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(x[c][e])), __uint_as_float(x[c][e + 1]));
+        for (int e = 2; e < 32; e += 2) mx[c] = max3(mx[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool grow = (top - m) * p.scale_log2 > kRescaleLog2;  // also the first finite score (m = -inf)

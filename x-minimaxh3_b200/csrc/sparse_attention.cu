@@ -34,7 +34,7 @@ bool encode_tmap_3d_bf16(CUtensorMap* map, const void* base, uint64_t d0, uint64
 
 namespace {
 
-constexpr int kSpThreads = 352;    // 2 x 4 softmax warps, TMA warp, one MMA warp per stream
+constexpr int kSpThreads = 384;    // 2 x 4 softmax warps, two TMA warps (8, 11), one MMA warp per stream (9, 10)
 constexpr int kSubKeys = 64;  // keys of one TMA box; a tile holds two
 constexpr int kTileBytes = 128 * kHeadDim * 2;     // 32 KB: a Q, K or V tile
 constexpr int kHalfBytes = kTileBytes / 2;         // dims 0..63 or 64..127 of 128 rows
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 1);
+      mbar_init(&q_full[i], 2);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 4);  // one arrival per softmax warp
       mbar_init(&p_full[2 * i + 1], 4);
@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_init(&turn[i], 1);
     }
     for (int i = 0; i < kRing; ++i) {
-      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_full[i], 2);  // one arrival per TMA warp
       mbar_init(&kv_empty[i], 1);
     }
     fence_barrier_init();
@@ -203,32 +203,31 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   const int n0 = tiles_of[0], n1 = tiles_of[1];
   const int nmax = max(n0, n1);
 
-  if (warp == 8) {
+  if (warp == 8 || warp == 11) {
     if (lane == 0) {
-      // ---------------- TMA producer: the order in which the MMA warp consumes ----------------
+      // ---------------- TMA producers: warp 8 loads the first 64 keys of each tile, 11 the second ----------------
+      // (one thread issues a 64-row box every 237 clocks, 34 B/clk, whatever is in flight;
+      // two threads reach 48 B/clk together). Both follow the order in which the MMA
+      // warps consume.
+      const int u = warp == 8 ? 0 : 1;
       int issued = 0;
       bool ok = true;
       const Stream st[2] = {stream_of(p, 0), stream_of(p, 1)};
       const int n[2] = {n0, n1};
       for (int s = 0; s < 2; ++s)
         if (n[s] > 0) {
-          mbar_arrive_expect_tx(&q_full[s], kTileBytes);
-          for (int h = 0; h < 2; ++h)
-            tma_load_3d(smem + s * kTileBytes + h * kHalfBytes, &tm_q, &q_full[s], h * 64, st[s].q_block * kQueryBlock,
-                        st[s].head);
+          mbar_arrive_expect_tx(&q_full[s], kHalfBytes);
+          tma_load_3d(smem + s * kTileBytes + u * kHalfBytes, &tm_q, &q_full[s], u * 64, st[s].q_block * kQueryBlock,
+                      st[s].head);
         }
       auto load_tile = [&](int s, int i, const CUtensorMap* map) {
         const int slot = issued % kRing;
-        const int key0 = sub_key(p, st[s].list, 2 * i), key1 = sub_key(p, st[s].list, 2 * i + 1);
+        const int key = sub_key(p, st[s].list, 2 * i + u);
         if (!mbar_wait(&kv_empty[slot], ((issued / kRing) & 1) ^ 1, kErrSpProd)) return false;
-        uint8_t* dst = smem + kOffRing + slot * kTileBytes;
-        mbar_arrive_expect_tx(&kv_full[slot], kTileBytes);
-        for (int u = 0; u < 2; ++u) {
-          const int key = u ? key1 : key0;
-          for (int h = 0; h < 2; ++h)  // rows past the last key (and absent sub-blocks) arrive as zeros
-            tma_load_3d(dst + h * kHalfBytes + u * (kSubKeys * 128), map, &kv_full[slot], h * 64,
-                        key < 0 ? p.keys : key, st[s].head / p.group);
-        }
+        uint8_t* dst = smem + kOffRing + slot * kTileBytes + u * (kSubKeys * 128);
+        mbar_arrive_expect_tx(&kv_full[slot], kHalfBytes);
+        for (int h = 0; h < 2; ++h)  // rows past the last key (and absent sub-blocks) arrive as zeros
+          tma_load_3d(dst + h * kHalfBytes, map, &kv_full[slot], h * 64, key < 0 ? p.keys : key, st[s].head / p.group);
         ++issued;
         return true;
       };

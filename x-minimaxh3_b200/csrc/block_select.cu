@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float*
                                                                     int64_t q_blocks, int k_blocks, int top_k,
                                                                     int rows_per_cta, int block, int64_t queries,
                                                                     int64_t keys, int causal,
-                                                                    int32_t* __restrict__ out) {
+                                                                    int32_t* __restrict__ out,
+                                                                    int32_t* __restrict__ out_tiles) {
   extern __shared__ __align__(16) unsigned char sel_smem[];
   double* qs = reinterpret_cast<double*>(sel_smem);                               // [rows][128]
   unsigned long long* key = reinterpret_cast<unsigned long long*>(qs + kSelRows * kHeadDim);  // [rows][k_blocks]
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float*
     equal_left -= __popc(equal & taken);
   }
   for (int j = at + lane; j < top_k; j += 32) dst[j] = -1;
+  if (out_tiles != nullptr && lane == 0) out_tiles[kvh * q_blocks + i0 + warp] = list_tiles(at, block / 64);
 }
 
 }  // namespace
@@ -267,7 +269,7 @@ cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream)
   if (grid > 0x7FFFFFFF) return cudaErrorNotSupported;
   select_blocks_kernel<<<(unsigned)grid, kSelThreads, smem, stream>>>(
       a.q_means, a.k_means, a.km_h, a.km_b, (int)(a.heads / a.kv_heads), a.q_blocks, (int)a.k_blocks, (int)a.top_k, rows, (int)a.block,
-      a.queries, a.keys, a.causal ? 1 : 0, a.out);
+      a.queries, a.keys, a.causal ? 1 : 0, a.out, a.tiles);
   return cudaGetLastError();
 }
 

@@ -1529,11 +1529,9 @@ int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t x_sh, int6
   return from_cuda(h3::launch_block_means(x, x_st, x_sh, tokens, heads, block, dtype == H3B200_DTYPE_F16, means, S(stream)), who);
 }
 
-int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb, int64_t heads,
-                             int64_t kv_heads, int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
-                             int32_t* blocks, h3b200_stream_t stream) {
-  H3_GUARD("select_key_blocks", stream);
-  const char* who = "select_key_blocks";
+static int select_impl(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb, int64_t heads,
+                       int64_t kv_heads, int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
+                       int32_t* blocks, int32_t* tiles, h3b200_stream_t stream, const char* who) {
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
   if (queries < 0 || keys < 0 || block <= 0 || block > (1 << 20) || top_k <= 0 || top_k > (1 << 24)) return fail(H3B200_ERR_INVALID, "%s: bad shape (top_k and block must be positive)", who);
   if (queries == 0) return H3B200_OK;
@@ -1544,24 +1542,31 @@ int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t
   a.q_means = q_means; a.k_means = k_means; a.km_h = km_sh; a.km_b = km_sb; a.heads = heads; a.kv_heads = kv_heads;
   a.q_blocks = (queries + h3::kQueryBlock - 1) / h3::kQueryBlock;
   a.k_blocks = k_blocks; a.top_k = top_k; a.block = block; a.queries = queries; a.keys = keys;
-  a.causal = causal != 0; a.out = blocks;
+  a.causal = causal != 0; a.out = blocks; a.tiles = tiles;
   return from_cuda(h3::launch_select_blocks(a, S(stream)), who);
+}
+
+int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb, int64_t heads,
+                             int64_t kv_heads, int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
+                             int32_t* blocks, h3b200_stream_t stream) {
+  H3_GUARD("select_key_blocks", stream);
+  return select_impl(q_means, k_means, km_sh, km_sb, heads, kv_heads, queries, keys, block, top_k, causal, blocks, nullptr, stream, "select_key_blocks");
 }
 
 int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k,
                                             int64_t block) {
-  if (queries != 1 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || top_k <= 0 || block <= 0) return 0;
-  return h3::paged_decode_workspace_bytes(1, heads, kv_heads, top_k * block, current_sms());
+  if (queries <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || top_k <= 0 || block <= 0) return 0;
+  if (queries == 1) return h3::paged_decode_workspace_bytes(1, heads, kv_heads, top_k * block, current_sms());
+  return h3::block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block, current_sms());
 }
 
-int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
-                                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks,
-                                  int64_t top_k, int64_t block, void* out, int64_t o_st, int64_t o_sh, float* lse,
-                                  int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys, int64_t heads,
-                                  int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
-                                  int64_t workspace_bytes, h3b200_stream_t stream) {
-  H3_GUARD("block_sparse_attention", stream);
-  const char* who = "block_sparse_attention";
+// tiles: h3::list_tiles of each list where the caller knows them, else nullptr
+static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                             const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks, const int32_t* tiles,
+                             int64_t top_k, int64_t block, void* out, int64_t o_st, int64_t o_sh, float* lse,
+                             int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys, int64_t heads,
+                             int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
+                             int64_t workspace_bytes, h3b200_stream_t stream, const char* who) {
   if (const int rc = attn_dtype(dtype, who)) return rc;
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
   if (queries < 0 || keys <= 0 || top_k <= 0) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys and top_k must be positive)", who);
@@ -1570,12 +1575,12 @@ int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, con
   if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(H3B200_ERR_INVALID, "%s: scale must be positive and finite", who);
   if (queries == 0) return H3B200_OK;
   if (!q || !k || !v || !blocks || !out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  const int64_t need = h3b200_block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block);
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
   if (queries == 1) {
     // one token sees every key it lists (its position is the last one): the split kernel
     // with the list as each head's page table
-    const int64_t need = h3b200_block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block);
-    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
-      return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
     h3::PagedDecodeArgs a;
     a.q = q; a.q_b = 0; a.q_h = q_sh;
     a.k = k; a.k_page = block * k_st; a.k_head = k_sh; a.k_row = k_st;
@@ -1590,12 +1595,23 @@ int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, con
   h3::SparseAttnArgs a;
   a.q = q; a.k = k; a.v = v;
   a.q_t = q_st; a.q_h = q_sh; a.k_t = k_st; a.k_h = k_sh; a.v_t = v_st; a.v_h = v_sh;
-  a.blocks = blocks;
+  a.blocks = blocks; a.tiles = tiles; a.workspace = workspace;
   a.queries = queries; a.keys = keys; a.heads = heads; a.kv_heads = kv_heads; a.top_k = top_k; a.block = block;
   a.scale = scale; a.causal = causal != 0;
   a.out = out; a.o_t = o_st; a.o_h = o_sh; a.lse = lse; a.l_t = l_st; a.l_h = l_sh;
   a.f16 = dtype == H3B200_DTYPE_F16;
   return from_cuda(h3::launch_block_sparse_attention(a, S(stream)), who);
+}
+
+int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                                  int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks,
+                                  int64_t top_k, int64_t block, void* out, int64_t o_st, int64_t o_sh, float* lse,
+                                  int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys, int64_t heads,
+                                  int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
+                                  int64_t workspace_bytes, h3b200_stream_t stream) {
+  H3_GUARD("block_sparse_attention", stream);
+  return block_sparse_impl(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, nullptr, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
+                           heads, kv_heads, scale, causal, dtype, workspace, workspace_bytes, stream, "block_sparse_attention");
 }
 
 int64_t h3b200_sparse_attention_workspace_bytes(int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
@@ -1632,9 +1648,11 @@ int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const voi
     if (const int rc = h3b200_attention_block_means(k, k_st, k_sh, keys, kv_heads, block, dtype, km, stream)) return rc;
     k_means = km; km_sh = k_blocks * h3::kHeadDim; km_sb = h3::kHeadDim;
   }
-  if (const int rc = h3b200_select_key_blocks(qm, k_means, km_sh, km_sb, heads, kv_heads, queries, keys, block, top_k, causal, blocks, stream)) return rc;
-  return h3b200_block_sparse_attention(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
-                                       heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, stream);
+  // the lists' tile counts go where the attention would count them
+  int32_t* tiles = queries > 1 ? reinterpret_cast<int32_t*>(base) : nullptr;
+  if (const int rc = select_impl(qm, k_means, km_sh, km_sb, heads, kv_heads, queries, keys, block, top_k, causal, blocks, tiles, stream, who)) return rc;
+  return block_sparse_impl(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, tiles, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
+                           heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, stream, who);
 }
 
 }  // extern "C"

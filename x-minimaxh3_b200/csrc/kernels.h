@@ -348,7 +348,10 @@ struct SelectBlocksArgs {
   int64_t heads = 0, kv_heads = 0, q_blocks = 0, k_blocks = 0, top_k = 0, block = 0, queries = 0, keys = 0;
   bool causal = false;
   int32_t* out = nullptr;
+  int32_t* tiles = nullptr;  // optional [kv_heads, q_blocks]: list_tiles of each list
 };
+// 128-key tiles of a list of `count` blocks
+__host__ __device__ inline int list_tiles(int count, int subs_per_block) { return (count * subs_per_block + 1) / 2; }
 int64_t select_blocks_max();  // key blocks the kernel can score
 cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream);
 
@@ -364,8 +367,12 @@ struct SparseAttnArgs {
   int64_t o_t = 0, o_h = 0;
   float* lse = nullptr;
   int64_t l_t = 0, l_h = 0;
+  const int32_t* tiles = nullptr;  // list_tiles of each list, where the caller knows them
+  void* workspace = nullptr;       // block_sparse_workspace_bytes, 16-byte aligned
   bool f16 = false;
 };
+int64_t block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k, int64_t block,
+                                     int sms);
 cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t stream);
 
 // 2-D tiled TMA descriptor (no interleave, 256-byte L2 promotion, no OOB fill);

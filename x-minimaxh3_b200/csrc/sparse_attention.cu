@@ -41,23 +41,34 @@ constexpr int kHalfBytes = kTileBytes / 2;         // dims 0..63 or 64..127 of 1
 constexpr int kRing = 5;
 constexpr int kOffRing = 2 * kTileBytes;
 constexpr int kOffBar = kOffRing + kRing * kTileBytes;
-constexpr int kSpSmem = kOffBar + 512 + 1024;      // + barriers + alignment
+constexpr int kSpSmem = kOffBar + 1024 + 1024;     // + barriers and notes + alignment
 constexpr unsigned kErrSpProd = 0x501, kErrSpMma = 0x502, kErrSpSoft = 0x503, kErrSpOut = 0x504, kErrSpDrain = 0x505;
 constexpr float kRescaleLog2 = 8.0f;
 
 struct SparseParams {
   const int32_t* blocks;  // [kv_heads, q_blocks, top_k]
+  const int32_t* tiles;   // [kv_heads, q_blocks]: tiles up to the list's last block
   int top_k, block, k_blocks;
   int queries, keys, q_blocks, heads, group;
-  int64_t items;
-  int streams;            // 2: the CTA's items are 2 b and 2 b + 1; 1: item b alone
+  int items, parts;       // items = heads * q_blocks * parts: a list is split into `parts` runs of tiles
   int causal;
+  float* ws_acc;          // parts > 1: unnormalised fp32 rows [items][128][128] and their (m, l)
+  float2* ws_ml;
   float scale, scale_log2;
   uint16_t* out;
   int64_t o_t, o_h;
+  int out32;              // rows of out are 32-byte aligned
   float* lse;
   int64_t l_t, l_h;
 };
+
+// one 32-byte sector per lane
+__device__ __forceinline__ void stg_v8(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d, uint32_t e, uint32_t f,
+                                       uint32_t g, uint32_t h) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a), "r"(b), "r"(c), "r"(d), "r"(e),
+               "r"(f), "r"(g), "r"(h)
+               : "memory");
+}
 
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int32_t x,
                                             int32_t y, int32_t z) {
@@ -125,20 +136,34 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 
-struct Stream {
-  int64_t item;
-  int head, q_block;
+// Item `idx`: tiles [first, first + n) of the list of one query block of one head.
+struct Work {
+  int head, q_block, part, first, n;
   const int32_t* list;
 };
 
-__device__ __forceinline__ Stream stream_of(const SparseParams& p, int s) {
-  Stream st;
-  st.item = p.streams == 2 ? (int64_t)blockIdx.x * 2 + s : (int64_t)blockIdx.x;
-  st.head = (int)(st.item / p.q_blocks);
-  st.q_block = (int)(st.item - (int64_t)st.head * p.q_blocks);
-  st.list = p.blocks + ((int64_t)(st.head / p.group) * p.q_blocks + st.q_block) * p.top_k;
-  return st;
+__device__ __forceinline__ Work work_of(const SparseParams& p, int idx) {
+  Work w;
+  const int row = idx / p.parts;
+  w.part = idx - row * p.parts;
+  w.head = row / p.q_blocks;
+  w.q_block = row - w.head * p.q_blocks;
+  if (p.causal) w.q_block = p.q_blocks - 1 - w.q_block;  // the longest lists first
+  const int at = (w.head / p.group) * p.q_blocks + w.q_block;
+  w.list = p.blocks + (int64_t)at * p.top_k;
+  const int total = __ldg(p.tiles + at);
+  const int per = (total + p.parts - 1) / p.parts;
+  w.first = min(total, w.part * per);
+  w.n = min(total - w.first, per);
+  return w;
 }
+
+// What the producers tell the other warps through shared memory (they run ahead by less
+// than the ring, so kNotes entries of each kind cannot be overtaken; the loads' barriers order them).
+constexpr int kNotes = 8;
+struct ItemNote {
+  int head, q_block, part, n;
+};
 
 template <bool F16>
 __global__ void __launch_bounds__(kSpThreads, 1)
@@ -148,19 +173,24 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   extern __shared__ uint8_t sp_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sp_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + kOffBar);  // [2]
-  uint64_t* kv_full = q_full + 2;                                  // [kRing]
+  uint64_t* q_empty = q_full + 2;                                  // [2] the item's last scores are computed
+  uint64_t* kv_full = q_empty + 2;                                 // [kRing]
   uint64_t* kv_empty = kv_full + kRing;                            // [kRing]
   uint64_t* s_full = kv_empty + kRing;                             // [2] scores are in TMEM
   uint64_t* p_full = s_full + 2;                                   // [2][2] a half of P is in TMEM, O is rescaled
-  uint64_t* o_full = p_full + 4;                                   // [2] O is complete
+  uint64_t* o_full = p_full + 4;                                   // [2] the item's O is complete
   uint64_t* turn = o_full + 2;                                     // [2] the stream's products of a tile are issued
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
-  int* tiles_of = reinterpret_cast<int*>(tmem_slot + 1);           // [2]
+  int* tiles_of = reinterpret_cast<int*>(tmem_slot + 1);           // [2] tiles of each stream
+  int* empty_of = tiles_of + 2;                                    // [2] whether it has items without tiles
+  ItemNote* item_note = reinterpret_cast<ItemNote*>(smem + kOffBar + 384);  // [2][kNotes] items that have tiles
+  int2* key_note = reinterpret_cast<int2*>(item_note + 2 * kNotes);         // [2][kNotes] first keys of a tile's halves
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&q_full[i], 2);
+      mbar_init(&q_full[i], 2);  // one arrival per TMA warp
+      mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[2 * i], 4);  // one arrival per softmax warp
       mbar_init(&p_full[2 * i + 1], 4);
@@ -177,22 +207,23 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
-  if (warp == 8) {
-    // tiles of each stream: up to its last listed block
-    for (int s = 0; s < 2; ++s) {
-      int last = -1;
-      if (s < p.streams && stream_of(p, s).item < p.items) {
-        const int32_t* list = stream_of(p, s).list;
-        for (int e = lane; e < p.top_k; e += 32) {
-          const int id = __ldg(list + e);
-          if (id >= 0 && id < p.k_blocks) last = e;
-        }
-      }
-      last = __reduce_max_sync(0xFFFFFFFFu, last);
-      if (lane == 0) tiles_of[s] = ((last + 1) * (p.block / kSubKeys) + 1) / 2;
+  if (warp == 8 || warp == 9) {
+    const int s = warp - 8;
+    int tiles = 0;
+    bool empty = false;
+    for (int idx = blockIdx.x + gridDim.x * (s + 2 * lane); idx < p.items; idx += 2 * 32 * gridDim.x) {
+      const int n = work_of(p, idx).n;
+      tiles += n;
+      empty = empty || n == 0;
+    }
+    tiles = (int)__reduce_add_sync(0xFFFFFFFFu, (unsigned)tiles);
+    empty = __any_sync(0xFFFFFFFFu, empty);
+    if (lane == 0) {
+      tiles_of[s] = tiles;
+      empty_of[s] = empty ? 1 : 0;
     }
   }
-  if (warp == 9) {
+  if (warp == 10) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -201,87 +232,164 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const int n0 = tiles_of[0], n1 = tiles_of[1];
-  const int nmax = max(n0, n1);
 
   if (warp == 8 || warp == 11) {
-    if (lane == 0) {
-      // ---------------- TMA producers: warp 8 loads the first 64 keys of each tile, 11 the second ----------------
-      // (one thread issues a 64-row box every 237 clocks, 34 B/clk, whatever is in flight;
-      // two threads reach 48 B/clk together). Both follow the order in which the MMA
-      // warps consume.
-      const int u = warp == 8 ? 0 : 1;
-      int issued = 0;
-      bool ok = true;
-      const Stream st[2] = {stream_of(p, 0), stream_of(p, 1)};
-      const int n[2] = {n0, n1};
-      for (int s = 0; s < 2; ++s)
-        if (n[s] > 0) {
-          mbar_arrive_expect_tx(&q_full[s], kHalfBytes);
-          tma_load_3d(smem + s * kTileBytes + u * kHalfBytes, &tm_q, &q_full[s], u * 64, st[s].q_block * kQueryBlock,
-                      st[s].head);
-        }
-      auto load_tile = [&](int s, int i, const CUtensorMap* map) {
-        const int slot = issued % kRing;
-        const int key = sub_key(p, st[s].list, 2 * i + u);
-        if (!mbar_wait(&kv_empty[slot], ((issued / kRing) & 1) ^ 1, kErrSpProd)) return false;
+    // ---------------- TMA producers: warp 8 loads the first 64 keys of each tile, 11 the second ----------------
+    // (one thread issues a 64-row box every 237 clocks, 34 B/clk, whatever is in flight;
+    // two threads reach 48 B/clk together). Both follow the order in which the MMA
+    // warps consume. The whole warp walks the lists, one lane per tile, so that an
+    // item costs one list read and a tile none.
+    const int u = warp == 8 ? 0 : 1;
+    int issued = 0;
+    bool ok = true;
+    struct Lane {
+      Work w;             // the item whose K tiles are being loaded, and the one after it
+      Work next;
+      int idx, i, item, ids0, ids1, v_key, v_head, tile;
+      bool more, pending; // more K tiles to load; V of the last K tile is not loaded yet
+    } st[2];
+    auto seek = [&](int idx, Work& w) {  // first item from idx on that has tiles
+      for (; idx < p.items; idx += 2 * gridDim.x) {
+        w = work_of(p, idx);
+        if (w.n > 0) break;
+      }
+      return idx;
+    };
+    auto read_ids = [&](Lane& t) {  // lane e: tile i + e
+      t.ids0 = t.ids1 = -1;
+      if (t.i + lane < t.w.n) {
+        t.ids0 = sub_key(p, t.w.list, 2 * (t.w.first + t.i + lane));
+        t.ids1 = sub_key(p, t.w.list, 2 * (t.w.first + t.i + lane) + 1);
+      }
+    };
+    auto load_tile = [&](int key, int kv_head, const CUtensorMap* map) {
+      const int slot = issued % kRing;
+      // one verdict for the warp: the shuffles below need all of it
+      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[slot], ((issued / kRing) & 1) ^ 1, kErrSpProd))) return false;
+      if (lane == 0) {
         uint8_t* dst = smem + kOffRing + slot * kTileBytes + u * (kSubKeys * 128);
         mbar_arrive_expect_tx(&kv_full[slot], kHalfBytes);
         for (int h = 0; h < 2; ++h)  // rows past the last key (and absent sub-blocks) arrive as zeros
-          tma_load_3d(dst + h * kHalfBytes, map, &kv_full[slot], h * 64, key < 0 ? p.keys : key, st[s].head / p.group);
-        ++issued;
-        return true;
-      };
-      for (int s = 0; s < 2 && ok; ++s)
-        if (n[s] > 0) ok = load_tile(s, 0, &tm_k);
-      for (int i = 0; i < nmax && ok; ++i)
-        for (int s = 0; s < 2 && ok; ++s) {
-          if (i < n[s]) ok = load_tile(s, i, &tm_v);
-          if (ok && i + 1 < n[s]) ok = load_tile(s, i + 1, &tm_k);
+          tma_load_3d(dst + h * kHalfBytes, map, &kv_full[slot], h * 64, key < 0 ? p.keys : key, kv_head);
+      }
+      ++issued;
+      return true;
+    };
+    auto load_k = [&](int s, Lane& t) {
+      if (t.i == 0) {  // a new item: its queries, once the item before has used the buffer
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&q_empty[s], (t.item & 1) ^ 1, kErrSpProd))) return false;
+        if (lane == 0) {
+          if (u == 0) item_note[s * kNotes + t.item % kNotes] = ItemNote{t.w.head, t.w.q_block, t.w.part, t.w.n};
+          mbar_arrive_expect_tx(&q_full[s], kHalfBytes);
+          tma_load_3d(smem + s * kTileBytes + u * kHalfBytes, &tm_q, &q_full[s], u * 64, t.w.q_block * kQueryBlock,
+                      t.w.head);
         }
-      for (int s = 0; s < 2; ++s)  // issued copies land before exit
-        if (n[s] > 0) mbar_wait(&q_full[s], 0, kErrSpDrain, 200000000ull);
-      for (int j = (issued > kRing ? issued - kRing : 0); j < issued; ++j)
-        mbar_wait(&kv_full[j % kRing], (j / kRing) & 1, kErrSpDrain, 200000000ull);
+        ++t.item;
+      }
+      const int key0 = __shfl_sync(0xFFFFFFFFu, t.ids0, t.i & 31), key1 = __shfl_sync(0xFFFFFFFFu, t.ids1, t.i & 31);
+      if (u == 0 && lane == 0) key_note[s * kNotes + t.tile % kNotes] = make_int2(key0, key1);
+      ++t.tile;
+      t.v_key = u == 0 ? key0 : key1;
+      t.v_head = t.w.head / p.group;
+      t.pending = true;
+      if (!load_tile(t.v_key, t.v_head, &tm_k)) return false;
+      if (++t.i == t.w.n) {
+        t.w = t.next;
+        t.i = 0;
+        t.more = t.idx < p.items;
+        if (t.more) {
+          read_ids(t);
+          t.idx = seek(t.idx + 2 * gridDim.x, t.next);
+        }
+      } else if ((t.i & 31) == 0) {
+        read_ids(t);
+      }
+      return true;
+    };
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      Lane& t = st[s];
+      t.i = t.item = t.tile = 0;
+      t.pending = false;
+      t.idx = seek(blockIdx.x + gridDim.x * s, t.w);
+      t.more = t.idx < p.items;
+      if (t.more) {
+        read_ids(t);
+        t.idx = seek(t.idx + 2 * gridDim.x, t.next);
+      }
     }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+      if (ok && st[s].more) ok = load_k(s, st[s]);
+    while (ok && (st[0].pending || st[1].pending)) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (!ok || !st[s].pending) continue;
+        st[s].pending = false;
+        ok = load_tile(st[s].v_key, st[s].v_head, &tm_v);
+        if (ok && st[s].more) ok = load_k(s, st[s]);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s)  // issued copies land before exit
+      if (st[s].item > 0) mbar_wait(&q_full[s], (st[s].item - 1) & 1, kErrSpDrain, 200000000ull);
+    for (int j = (issued > kRing ? issued - kRing : 0); j < issued; ++j)
+      mbar_wait(&kv_full[j % kRing], (j / kRing) & 1, kErrSpDrain, 200000000ull);
   } else if (warp >= 9) {
     if (lane == 0) {
       // ---------------- MMA issuers: warp 9 + s serves stream s ----------------
       // An issuing thread is held until its instruction enters the (short) tensor queue,
       // so its waits for softmax and loads would leave the tensor core idle; with an
       // issuer per stream they run beside the other stream's products. The issuers take
-      // turns (turn[s]: stream s has issued its i-th P V and next Q K^T): left to
+      // turns (turn[s]: stream s has issued its t-th P V and next Q K^T): left to
       // themselves they interleave instruction by instruction, both softmaxes then start
       // together, and the exponentials of one no longer hide behind the products of the
       // other (2,126 us on the 21 x 39 x 40 grid, 24 heads, 64 of 512 blocks). Ring slots
-      // keep the producer's order over both streams: an issuer counts past the other's tiles.
+      // keep the producers' order over both streams: an issuer counts past the other's tiles.
       constexpr uint32_t kIdescS = idesc_f16kind(F16, false), kIdescO = idesc_f16kind(F16, true);
       const int s = warp - 9, n = s ? n1 : n0, other = s ? n0 : n1;
       const uint32_t t_s = tmem + s * 128, t_o = tmem + 256 + s * 128;
       const uint64_t q_desc = umma_desc_sw128(smem_u32(smem + s * kTileBytes));
       const uint32_t ring = smem_u32(smem + kOffRing);
       int at = s == 1 && other > 0 ? 1 : 0;  // ring position of this stream's next tile
-      auto scores = [&]() {
-        const int slot = at % kRing;
+      int item = 0;                          // items whose scores have begun
+      int opens = 1, left_s = 0;             // the next scores open an item; its tiles whose scores are to come
+      auto loaded = [&](int pos) { return mbar_wait(&kv_full[pos % kRing], (pos / kRing) & 1, kErrSpMma); };
+      auto queries_loaded = [&]() {
+        if (!opens) return true;
+        ++item;
+        return mbar_wait(&q_full[s], (item - 1) & 1, kErrSpMma);
+      };
+      // scores of the next tile from ring position pos; `pass`: hand the turn over on the way
+      auto scores = [&](int pos, bool pass) {
+        const int slot = pos % kRing;
+        if (opens) left_s = item_note[s * kNotes + (item - 1) % kNotes].n;
+        opens = --left_s == 0;
         const uint64_t k_desc = umma_desc_sw128(ring + slot * kTileBytes);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint32_t off = ((k >> 2) * kHalfBytes + (k & 3) * 32) >> 4;
           umma_bf16(t_s, q_desc + off, k_desc + off, kIdescS, k > 0 ? 1u : 0u);
+          if (pass && k == 5) mbar_arrive(&turn[s]);  // the other issuer wakes while the last ones run
         }
         umma_commit(&s_full[s]);
         umma_commit(&kv_empty[slot]);
+        if (opens) umma_commit(&q_empty[s]);  // the item's last scores
       };
-      bool ok = n > 0 && mbar_wait(&q_full[s], 0, kErrSpMma) &&
-                mbar_wait(&kv_full[at % kRing], (at / kRing) & 1, kErrSpMma);
+      bool ok = n > 0 && queries_loaded() && loaded(at);
+      int left = 0;  // tiles of the current item whose P V is not issued
       if (ok) {
         tc_fence_after();
-        scores();
+        scores(at, false);
+        left = left_s + 1;
       }
       at = (n0 > 0 ? 1 : 0) + (n1 > 0 ? 1 : 0) + (s == 1 ? (other > 0 ? 1 : 0) + (other > 1 ? 1 : 0) : 0);
+      bool first = true;  // of its item
       for (int i = 0; i < n && ok; ++i) {
         const int slot = at % kRing;
-        ok = mbar_wait(&kv_full[slot], (at / kRing) & 1, kErrSpMma);
-        if (i + 1 < n) ok = ok && mbar_wait(&kv_full[(at + 1) % kRing], ((at + 1) / kRing) & 1, kErrSpMma);
+        const bool more = i + 1 < n;
+        ok = loaded(at);
+        if (more) ok = ok && queries_loaded() && loaded(at + 1);
         ok = ok && mbar_wait(&p_full[2 * s], i & 1, kErrSpMma);
         const int before = s == 0 ? i - 1 : i;  // the other stream's tile whose turn comes first
         if (before >= 0 && before < other) ok = ok && mbar_wait(&turn[1 - s], before & 1, kErrSpMma);
@@ -293,48 +401,48 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           tc_fence_after();
 #pragma unroll
           for (int k = 4 * h; k < 4 * h + 4; ++k)
-            umma_f16_ts(t_o, t_s + k * 8, v_desc + ((k * 16 * 128) >> 4), kIdescO, i > 0 || k > 0 ? 1u : 0u);
+            umma_f16_ts(t_o, t_s + k * 8, v_desc + ((k * 16 * 128) >> 4), kIdescO, !first || k > 0 ? 1u : 0u);
         }
         if (!ok) break;
-        if (i + 1 < n) {
-          ++at;
-          scores();  // executes after the product above, which reads the columns it overwrites
-          // then the other stream's V and next K: tile i of stream 1, tile i + 1 of stream 0
+        first = --left == 0;  // the next tile opens an item
+        if (first) umma_commit(&o_full[s]);
+        if (more) {
+          scores(at + 1, true);  // executes after the product above, which reads the columns it overwrites
+          if (first) left = left_s + 1;
+          // V and next K of this tile, then the other stream's: its tile i (stream 1) or i + 1 (stream 0)
           const int j = s == 0 ? i : i + 1;
-          at += 1 + (j < other ? 1 : 0) + (j + 1 < other ? 1 : 0);
+          at += 2 + (j < other ? 1 : 0) + (j + 1 < other ? 1 : 0);
         } else {
-          umma_commit(&o_full[s]);
+          mbar_arrive(&turn[s]);
         }
-        mbar_arrive(&turn[s]);
         umma_commit(&kv_empty[slot]);
       }
     }
   } else {
     // ---------------- softmax: thread = row ----------------
     const int s = warp >> 2;
-    const int n = s ? n1 : n0;
-    const Stream st = stream_of(p, s);
-    const int row = st.q_block * kQueryBlock + (warp & 3) * 32 + lane;
+    const int row_in = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + s * 128 + lanes;
-    const int limit = p.causal ? min(p.keys, row + 1 + p.keys - p.queries) : p.keys;  // keys this row may see
+    const int total = s ? n1 : n0;
+    ItemNote it;
+    int i = 0, item = 0, row = 0, limit = 0;  // limit: keys this row may see
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
-    int key0 = -1, key1 = -1;
-    if (n > 0) {
-      key0 = sub_key(p, st.list, 0);
-      key1 = sub_key(p, st.list, 1);
-    }
-    for (int i = 0; i < n; ++i) {
-      const int v0 = key0 < 0 ? 0 : limit - key0, v1 = key1 < 0 ? 0 : limit - key1;  // visible keys of the halves
-      if (i + 1 < n) {
-        key0 = sub_key(p, st.list, 2 * i + 2);
-        key1 = sub_key(p, st.list, 2 * i + 3);
-      }
-      if (!mbar_wait(&s_full[s], i & 1, kErrSpSoft)) {
+    for (int t = 0; t < total; ++t) {
+      if (!mbar_wait(&s_full[s], t & 1, kErrSpSoft)) {
         ok = false;
         break;
       }
+      if (i == 0) {
+        it = item_note[s * kNotes + item % kNotes];
+        row = it.q_block * kQueryBlock + row_in;
+        limit = p.causal ? min(p.keys, row + 1 + p.keys - p.queries) : p.keys;
+        m = -INFINITY;
+        l = 0.0f;
+      }
+      const int2 key = key_note[s * kNotes + t % kNotes];
+      const int v0 = key.x < 0 ? 0 : limit - key.x, v1 = key.y < 0 ? 0 : limit - key.y;  // visible keys of the halves
       tc_fence_after();
       uint32_t x[4][32];
 #pragma unroll
@@ -400,45 +508,129 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       f2_unpack(sum[0], s0, s1);
       f2_unpack(sum[1], s2, s3);
       l += (s0 + s1) + (s2 + s3);
-    }
-    if (st.item < p.items && s < p.streams && ok) {
-      if (n > 0) ok = mbar_wait(&o_full[s], 0, kErrSpOut);
+      if (++i < it.n) continue;
+      // the item's last tile: its rows
+      if (!mbar_wait(&o_full[s], item & 1, kErrSpOut)) {
+        ok = false;
+        break;
+      }
       tc_fence_after();
-      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays
-      uint16_t* dst = p.out + (int64_t)row * p.o_t + (int64_t)st.head * p.o_h;
-      if (ok) {
-#pragma unroll
+      i = 0;
+      ++item;
+      if (p.parts > 1) {
+        const int64_t at = ((int64_t)(it.head * p.q_blocks + it.q_block) * p.parts + it.part) * kQueryBlock + row_in;
+        if (row < p.queries) p.ws_ml[at] = make_float2(m, l);
+#pragma unroll 2
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
-          if (n > 0) {
-            tmem_ld32(t_o + c * 32, o);
-            tmem_wait_ld();
-          }
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
           if (row < p.queries) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w[4];
+            for (int e = 0; e < 32; e += 8)
+              stg_v8(p.ws_acc + at * kHeadDim + c * 32 + e, o[e], o[e + 1], o[e + 2], o[e + 3], o[e + 4], o[e + 5],
+                     o[e + 6], o[e + 7]);
+          }
+          __syncwarp();
+        }
+      } else {
+        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays
+        uint16_t* dst = p.out + (int64_t)row * p.o_t + (int64_t)it.head * p.o_h;
+#pragma unroll 2
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32], w[16];
+          tmem_ld32(t_o + c * 32, o);
+          tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int at = e * 8 + 2 * j;
-                w[j] = l == 0.0f ? 0u : E::pack(__uint_as_float(o[at]) * inv, __uint_as_float(o[at + 1]) * inv);
-              }
-              stg_v4(dst + c * 32 + e * 8, make_uint4(w[0], w[1], w[2], w[3]));
+          for (int j = 0; j < 16; ++j)
+            w[j] = l == 0.0f ? 0u : E::pack(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
+          if (row < p.queries) {
+            if (p.out32) {
+              stg_v8(dst + c * 32, w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]);
+              stg_v8(dst + c * 32 + 16, w[8], w[9], w[10], w[11], w[12], w[13], w[14], w[15]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4) stg_v4(dst + c * 32 + 2 * e, make_uint4(w[e], w[e + 1], w[e + 2], w[e + 3]));
             }
           }
           __syncwarp();
         }
         if (row < p.queries && p.lse != nullptr)
-          p.lse[(int64_t)row * p.l_t + (int64_t)st.head * p.l_h] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l));
+          p.lse[(int64_t)row * p.l_t + (int64_t)it.head * p.l_h] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l));
+      }
+    }
+    if (ok && empty_of[s]) {  // query blocks without any key
+      for (int idx = blockIdx.x + gridDim.x * s; idx < p.items; idx += 2 * gridDim.x) {
+        const Work w = work_of(p, idx);
+        const int r = w.q_block * kQueryBlock + row_in;
+        if (w.n > 0 || r >= p.queries) continue;
+        if (p.parts > 1) {  // a part without tiles: l is 0, and the join reads no row
+          p.ws_ml[((int64_t)(w.head * p.q_blocks + w.q_block) * p.parts + w.part) * kQueryBlock + row_in] =
+              make_float2(-INFINITY, 0.0f);
+          continue;
+        }
+        uint16_t* dst = p.out + (int64_t)r * p.o_t + (int64_t)w.head * p.o_h;
+        for (int c = 0; c < kHeadDim; c += 8) stg_v4(dst + c, make_uint4(0u, 0u, 0u, 0u));
+        if (p.lse != nullptr) p.lse[(int64_t)r * p.l_t + (int64_t)w.head * p.l_h] = -INFINITY;
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 10) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// tiles[row] of each list: up to its last block that exists
+__global__ void __launch_bounds__(128) count_tiles_kernel(const int32_t* blocks, int64_t rows, int top_k, int k_blocks,
+                                                          int subs_per_block, int32_t* tiles) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  int last = -1;
+  for (int e = lane; e < top_k; e += 32) {
+    const int id = __ldg(blocks + row * top_k + e);
+    if (id >= 0 && id < k_blocks) last = e;
+  }
+  last = __reduce_max_sync(0xFFFFFFFFu, last);
+  if (lane == 0) tiles[row] = list_tiles(last + 1, subs_per_block);
+}
+
+// Joins the parts of a query row: one warp per (row, head), in the order of the parts.
+template <bool F16>
+__global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) {
+  using E = Elem16<F16>;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (at >= (int64_t)p.heads * p.queries) return;
+  const int lane = threadIdx.x & 31;
+  const int head = (int)(at / p.queries), row = (int)(at - (int64_t)head * p.queries);
+  const int64_t first = ((int64_t)(head * p.q_blocks + row / kQueryBlock) * p.parts) * kQueryBlock + row % kQueryBlock;
+  float mx = -INFINITY;
+  for (int s = lane; s < p.parts; s += 32) mx = fmaxf(mx, p.ws_ml[first + (int64_t)s * kQueryBlock].x);
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, i));
+  float sum = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = 0; s < p.parts; ++s) {
+    const float2 ml = p.ws_ml[first + (int64_t)s * kQueryBlock];
+    if (ml.y == 0.0f) continue;  // no keys: nothing was written
+    const float f = ex2_approx((ml.x - mx) * p.scale_log2);
+    const float4 a = *(reinterpret_cast<const float4*>(p.ws_acc + (first + (int64_t)s * kQueryBlock) * kHeadDim) + lane);
+    sum = fmaf(ml.y, f, sum);
+    o.x = fmaf(a.x, f, o.x);
+    o.y = fmaf(a.y, f, o.y);
+    o.z = fmaf(a.z, f, o.z);
+    o.w = fmaf(a.w, f, o.w);
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+  uint2 y;
+  y.x = E::pack(o.x * inv, o.y * inv);
+  y.y = E::pack(o.z * inv, o.w * inv);
+  *reinterpret_cast<uint2*>(p.out + (int64_t)row * p.o_t + (int64_t)head * p.o_h + lane * 4) = y;
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[(int64_t)row * p.l_t + (int64_t)head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum));
 }
 
 bool map_view(CUtensorMap* map, const void* base, int64_t rows, int64_t heads, int64_t st, int64_t sh, int box_rows) {
@@ -461,35 +653,83 @@ cudaError_t launch_sparse(const CUtensorMap& q, const CUtensorMap& k, const CUte
     attr_set[dev] = true;
   }
   sparse_attention_kernel<F16><<<grid, kSpThreads, kSpSmem, stream>>>(q, k, v, p);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || p.parts == 1) return e;
+  const int64_t warps = (int64_t)p.heads * p.queries;
+  sparse_join_kernel<F16><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(p);
   return cudaGetLastError();
+}
+
+// Runs a list is split into: as many as fill the streams of all SMs, of at least two tiles.
+int64_t list_parts(int64_t items, int64_t tiles, int sms) {
+  return std::max<int64_t>(1, std::min<int64_t>(tiles / 2, 2 * sms / items));
+}
+
+struct SparseShape {
+  int64_t q_blocks, items, tiles, parts, tiles_bytes, acc_bytes, ml_bytes;
+};
+SparseShape sparse_shape(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k, int64_t block, int sms) {
+  SparseShape s;
+  s.q_blocks = (queries + kQueryBlock - 1) / kQueryBlock;
+  s.items = heads * s.q_blocks;
+  s.tiles = (top_k * block + 127) / 128;
+  s.parts = list_parts(s.items, s.tiles, sms);
+  const int64_t rows = s.parts > 1 ? s.items * s.parts * kQueryBlock : 0;
+  s.tiles_bytes = (kv_heads * s.q_blocks * 4 + 255) / 256 * 256;
+  s.acc_bytes = rows * kHeadDim * 4;
+  s.ml_bytes = rows * 8;
+  return s;
 }
 
 }  // namespace
 
+int64_t block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k, int64_t block,
+                                     int sms) {
+  const SparseShape s = sparse_shape(queries, heads, kv_heads, top_k, block, sms);
+  return s.tiles_bytes + s.acc_bytes + s.ml_bytes;
+}
+
 cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t stream) {
   if (a.queries <= 0 || a.heads <= 0) return cudaSuccess;
-  SparseParams p;
-  p.q_blocks = (int)((a.queries + kQueryBlock - 1) / kQueryBlock);
-  p.items = a.heads * p.q_blocks;
-  if (a.queries > 0x7FFFFF00 || a.keys > 0x7FFFFF00 || p.items > 0x7FFFFFFF || a.block % kSubKeys || a.o_t % 8 ||
-      a.o_h % 8 || (reinterpret_cast<uintptr_t>(a.out) & 15))
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int sms = num_sms(dev);
+  const SparseShape sh = sparse_shape(a.queries, a.heads, a.kv_heads, a.top_k, a.block, sms);
+  if (a.queries > 0x7FFFFF00 || a.keys > 0x7FFFFF00 || sh.items * sh.parts > (1 << 30) || a.block % kSubKeys ||
+      a.o_t % 8 || a.o_h % 8 || (reinterpret_cast<uintptr_t>(a.out) & 15))
     return cudaErrorNotSupported;
   CUtensorMap q, k, v;
   if (!map_view(&q, a.q, a.queries, a.heads, a.q_t, a.q_h, kQueryBlock) ||
       !map_view(&k, a.k, a.keys, a.kv_heads, a.k_t, a.k_h, kSubKeys) ||
       !map_view(&v, a.v, a.keys, a.kv_heads, a.v_t, a.v_h, kSubKeys))
     return cudaErrorNotSupported;
+  SparseParams p;
+  p.q_blocks = (int)sh.q_blocks;
+  p.parts = (int)sh.parts;
+  p.items = (int)(sh.items * sh.parts);
   p.blocks = a.blocks; p.top_k = (int)a.top_k; p.block = (int)a.block;
   p.k_blocks = (int)((a.keys + a.block - 1) / a.block);
   p.queries = (int)a.queries; p.keys = (int)a.keys; p.heads = (int)a.heads; p.group = (int)(a.heads / a.kv_heads);
   p.causal = a.causal ? 1 : 0;
   p.scale = a.scale; p.scale_log2 = a.scale * 1.4426950408889634f;
   p.out = static_cast<uint16_t*>(a.out); p.o_t = a.o_t; p.o_h = a.o_h;
+  p.out32 = ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)(a.o_t * 2) | (uintptr_t)(a.o_h * 2)) & 31) == 0;
   p.lse = a.lse; p.l_t = a.l_t; p.l_h = a.l_h;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  p.streams = p.items > num_sms(dev) ? 2 : 1;  // a second stream only where every SM has a first one
-  const unsigned grid = (unsigned)((p.items + p.streams - 1) / p.streams);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  p.ws_acc = reinterpret_cast<float*>(ws + sh.tiles_bytes);
+  p.ws_ml = reinterpret_cast<float2*>(ws + sh.tiles_bytes + sh.acc_bytes);
+  p.tiles = a.tiles;
+  if (p.tiles == nullptr) {
+    int32_t* tiles = reinterpret_cast<int32_t*>(ws);
+    const int64_t rows = a.kv_heads * sh.q_blocks;
+    count_tiles_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a.blocks, rows, p.top_k, p.k_blocks,
+                                                                      p.block / kSubKeys, tiles);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    p.tiles = tiles;
+  }
+  // one persistent CTA per SM; a second stream only where every SM has a first one
+  const unsigned grid = (unsigned)std::min<int64_t>(sms, p.items);
   return a.f16 ? launch_sparse<true>(q, k, v, p, grid, dev, stream) : launch_sparse<false>(q, k, v, p, grid, dev, stream);
 }
 

@@ -242,29 +242,69 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     const int u = warp == 8 ? 0 : 1;
     int issued = 0;
     bool ok = true;
-    struct Lane {
-      Work w;             // the item whose K tiles are being loaded, and the one after it
-      Work next;
-      int idx, i, item, ids0, ids1, v_key, v_head, tile;
-      bool more, pending; // more K tiles to load; V of the last K tile is not loaded yet
-    } st[2];
-    auto seek = [&](int idx, Work& w) {  // first item from idx on that has tiles
-      for (; idx < p.items; idx += 2 * gridDim.x) {
-        w = work_of(p, idx);
-        if (w.n > 0) break;
+    struct Feed {  // one stream
+      int s, base;                             // lane e of the batch: item base + e of the stream
+      int b_head, b_block, b_part, b_first, b_n;
+      int pos;                                 // the batch's next item
+      int n_head, n_block, n_part, n_first, n_n, n_ids0, n_ids1;  // the item after the current one (n_n 0: none)
+      int head, block, part, first, n;         // the item whose K tiles are being loaded (n 0: none)
+      int ids0, ids1;                          // lane e: keys of its tile i0 + e, i0 = i rounded down to 32
+      int i, item, tile, v_key, v_head;
+      bool pending;                            // V of the last K tile is not loaded yet
+    } a, o;
+    auto refill = [&](Feed& t) {
+      const int64_t idx = blockIdx.x + (int64_t)gridDim.x * (t.s + 2 * (int64_t)(t.base + lane));
+      t.b_n = -1;
+      if (idx < p.items) {
+        const Work w = work_of(p, (int)idx);
+        t.b_head = w.head; t.b_block = w.q_block; t.b_part = w.part; t.b_first = w.first; t.b_n = w.n;
       }
-      return idx;
+      t.pos = 0;
     };
-    auto read_ids = [&](Lane& t) {  // lane e: tile i + e
-      t.ids0 = t.ids1 = -1;
-      if (t.i + lane < t.w.n) {
-        t.ids0 = sub_key(p, t.w.list, 2 * (t.w.first + t.i + lane));
-        t.ids1 = sub_key(p, t.w.list, 2 * (t.w.first + t.i + lane) + 1);
+    auto read_ids = [&](int head, int block, int first, int n, int i, int& ids0, int& ids1) {
+      ids0 = ids1 = -1;
+      if (i + lane < n) {
+        const int32_t* list = p.blocks + (int64_t)((head / p.group) * p.q_blocks + block) * p.top_k;
+        ids0 = sub_key(p, list, 2 * (first + i + lane));
+        ids1 = sub_key(p, list, 2 * (first + i + lane) + 1);
       }
+    };
+    auto advance = [&](Feed& t) {  // the next item becomes the current one; the one after it is looked up
+      t.head = t.n_head; t.block = t.n_block; t.part = t.n_part; t.first = t.n_first; t.n = t.n_n;
+      t.ids0 = t.n_ids0; t.ids1 = t.n_ids1;
+      t.i = 0;
+      t.n_n = 0;
+      for (;;) {
+        if (t.pos == 32) {
+          t.base += 32;
+          refill(t);
+        }
+        const int n = __shfl_sync(0xFFFFFFFFu, t.b_n, t.pos);
+        if (n < 0) return;  // behind the last item
+        if (n > 0) break;
+        ++t.pos;
+      }
+      t.n_n = __shfl_sync(0xFFFFFFFFu, t.b_n, t.pos);
+      t.n_head = __shfl_sync(0xFFFFFFFFu, t.b_head, t.pos);
+      t.n_block = __shfl_sync(0xFFFFFFFFu, t.b_block, t.pos);
+      t.n_part = __shfl_sync(0xFFFFFFFFu, t.b_part, t.pos);
+      t.n_first = __shfl_sync(0xFFFFFFFFu, t.b_first, t.pos);
+      ++t.pos;
+      read_ids(t.n_head, t.n_block, t.n_first, t.n_n, 0, t.n_ids0, t.n_ids1);  // used an item later
+    };
+    auto start = [&](Feed& t, int s) {
+      t.s = s;
+      t.base = 0;
+      t.item = t.tile = 0;
+      t.pending = false;
+      refill(t);
+      t.n_n = 0;
+      advance(t);
+      advance(t);
     };
     auto load_tile = [&](int key, int kv_head, const CUtensorMap* map) {
       const int slot = issued % kRing;
-      // one verdict for the warp: the shuffles below need all of it
+      // one verdict for the warp: the shuffles need all of it
       if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[slot], ((issued / kRing) & 1) ^ 1, kErrSpProd))) return false;
       if (lane == 0) {
         uint8_t* dst = smem + kOffRing + slot * kTileBytes + u * (kSubKeys * 128);
@@ -275,64 +315,50 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       ++issued;
       return true;
     };
-    auto load_k = [&](int s, Lane& t) {
+    auto load_k = [&](Feed& t) {
       if (t.i == 0) {  // a new item: its queries, once the item before has used the buffer
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&q_empty[s], (t.item & 1) ^ 1, kErrSpProd))) return false;
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&q_empty[t.s], (t.item & 1) ^ 1, kErrSpProd))) return false;
         if (lane == 0) {
-          if (u == 0) item_note[s * kNotes + t.item % kNotes] = ItemNote{t.w.head, t.w.q_block, t.w.part, t.w.n};
-          mbar_arrive_expect_tx(&q_full[s], kHalfBytes);
-          tma_load_3d(smem + s * kTileBytes + u * kHalfBytes, &tm_q, &q_full[s], u * 64, t.w.q_block * kQueryBlock,
-                      t.w.head);
+          if (u == 0) item_note[t.s * kNotes + t.item % kNotes] = ItemNote{t.head, t.block, t.part, t.n};
+          mbar_arrive_expect_tx(&q_full[t.s], kHalfBytes);
+          tma_load_3d(smem + t.s * kTileBytes + u * kHalfBytes, &tm_q, &q_full[t.s], u * 64, t.block * kQueryBlock,
+                      t.head);
         }
         ++t.item;
       }
       const int key0 = __shfl_sync(0xFFFFFFFFu, t.ids0, t.i & 31), key1 = __shfl_sync(0xFFFFFFFFu, t.ids1, t.i & 31);
-      if (u == 0 && lane == 0) key_note[s * kNotes + t.tile % kNotes] = make_int2(key0, key1);
+      if (u == 0 && lane == 0) key_note[t.s * kNotes + t.tile % kNotes] = make_int2(key0, key1);
       ++t.tile;
       t.v_key = u == 0 ? key0 : key1;
-      t.v_head = t.w.head / p.group;
+      t.v_head = t.head / p.group;
       t.pending = true;
       if (!load_tile(t.v_key, t.v_head, &tm_k)) return false;
-      if (++t.i == t.w.n) {
-        t.w = t.next;
-        t.i = 0;
-        t.more = t.idx < p.items;
-        if (t.more) {
-          read_ids(t);
-          t.idx = seek(t.idx + 2 * gridDim.x, t.next);
-        }
-      } else if ((t.i & 31) == 0) {
-        read_ids(t);
-      }
+      if (++t.i == t.n)
+        advance(t);
+      else if ((t.i & 31) == 0)
+        read_ids(t.head, t.block, t.first, t.n, t.i, t.ids0, t.ids1);
       return true;
     };
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      Lane& t = st[s];
-      t.i = t.item = t.tile = 0;
-      t.pending = false;
-      t.idx = seek(blockIdx.x + gridDim.x * s, t.w);
-      t.more = t.idx < p.items;
-      if (t.more) {
-        read_ids(t);
-        t.idx = seek(t.idx + 2 * gridDim.x, t.next);
+    start(a, 0);
+    start(o, 1);
+    // K of both streams' first tiles, then V and the next K of one stream after the other
+#pragma unroll 1
+    while (ok && (a.pending || a.n > 0 || o.pending || o.n > 0)) {
+      if (a.pending) {
+        a.pending = false;
+        ok = load_tile(a.v_key, a.v_head, &tm_v);
       }
+      if (ok && a.n > 0) ok = load_k(a);
+      const Feed t = a;
+      a = o;
+      o = t;
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-      if (ok && st[s].more) ok = load_k(s, st[s]);
-    while (ok && (st[0].pending || st[1].pending)) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        if (!ok || !st[s].pending) continue;
-        st[s].pending = false;
-        ok = load_tile(st[s].v_key, st[s].v_head, &tm_v);
-        if (ok && st[s].more) ok = load_k(s, st[s]);
-      }
+#pragma unroll 1
+    for (int j = 0; j < 2; ++j) {  // issued copies land before exit
+      const Feed& t = j ? o : a;
+      if (t.item > 0) mbar_wait(&q_full[t.s], (t.item - 1) & 1, kErrSpDrain, 200000000ull);
     }
-#pragma unroll
-    for (int s = 0; s < 2; ++s)  // issued copies land before exit
-      if (st[s].item > 0) mbar_wait(&q_full[s], (st[s].item - 1) & 1, kErrSpDrain, 200000000ull);
+#pragma unroll 1
     for (int j = (issued > kRing ? issued - kRing : 0); j < issued; ++j)
       mbar_wait(&kv_full[j % kRing], (j / kRing) & 1, kErrSpDrain, 200000000ull);
   } else if (warp >= 9) {
@@ -444,23 +470,38 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const int2 key = key_note[s * kNotes + t % kNotes];
       const int v0 = key.x < 0 ? 0 : limit - key.x, v1 = key.y < 0 ? 0 : limit - key.y;  // visible keys of the halves
       tc_fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(t_s + c * 32, x[c]);
-      tmem_wait_ld();
       if (!__all_sync(0xFFFFFFFFu, v0 >= kSubKeys && v1 >= kSubKeys)) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
+        // keys this row may not see: -inf, written back
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const int seen = (c < 2 ? v0 : v1) - (c & 1) * 32;
+          uint32_t x[32];
+          tmem_ld32(t_s + c * 32, x);
+          tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            if ((c & 1) * 32 + e >= (c < 2 ? v0 : v1)) x[c][e] = 0xFF800000u;  // -inf
+            if (e >= seen) x[e] = 0xFF800000u;
+          tmem_st32(t_s + c * 32, x);
+        }
+        tmem_wait_st();
       }
-      float mx[4];
+      // Two passes over the row, the second reading the scores again: TMEM is read in
+      // some 50 clocks, and short loops instead of 128 scores in registers keep the code
+      // small (unrolled, the warps waited for instructions).
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+      for (int c = 0; c < 2; ++c) {
+        uint32_t x[2][32];
+        tmem_ld32(t_s + c * 64, x[0]);
+        tmem_ld32(t_s + c * 64 + 32, x[1]);
+        tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        mx[c] = fmaxf(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]));
-#pragma unroll
-        for (int e = 2; e < 32; e += 2) mx[c] = max3(mx[c], __uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1]));
+        for (int e = 0; e < 32; e += 4) {
+          mx[0] = max3(mx[0], __uint_as_float(x[0][e]), __uint_as_float(x[0][e + 1]));
+          mx[1] = max3(mx[1], __uint_as_float(x[0][e + 2]), __uint_as_float(x[0][e + 3]));
+          mx[2] = max3(mx[2], __uint_as_float(x[1][e]), __uint_as_float(x[1][e + 1]));
+          mx[3] = max3(mx[3], __uint_as_float(x[1][e + 2]), __uint_as_float(x[1][e + 3]));
+        }
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool grow = (top - m) * p.scale_log2 > kRescaleLog2;  // also the first finite score (m = -inf)
@@ -484,25 +525,27 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       const float sub = m == -INFINITY ? 0.0f : m * p.scale_log2;
       const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(-sub, -sub);
       uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        uint32_t x[2][32], w[32];
+        tmem_ld32(t_s + h * 64, x[0]);
+        tmem_ld32(t_s + h * 64 + 32, x[1]);
+        tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 32; ++e) {
+          const uint32_t* y = &x[e >> 4][2 * (e & 15)];
           float a, b;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1])), scale2, sub2), a, b);
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(y[0]), __uint_as_float(y[1])), scale2, sub2), a, b);
           a = ex2_approx(a);
           b = ex2_approx(b);
           sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, b));
           w[e] = E::pack(a, b);
         }
-        tmem_st16(t_s + c * 16, w);  // over columns already read
-        if (c & 1) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[2 * s + (c >> 1)]);
-        }
+        tmem_st32(t_s + h * 32, w);  // over columns already read
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
       }
       float s0, s1, s2, s3;
       f2_unpack(sum[0], s0, s1);
@@ -520,7 +563,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       if (p.parts > 1) {
         const int64_t at = ((int64_t)(it.head * p.q_blocks + it.q_block) * p.parts + it.part) * kQueryBlock + row_in;
         if (row < p.queries) p.ws_ml[at] = make_float2(m, l);
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32];
           tmem_ld32(t_o + c * 32, o);
@@ -536,7 +579,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       } else {
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);  // NaN stays
         uint16_t* dst = p.out + (int64_t)row * p.o_t + (int64_t)it.head * p.o_h;
-#pragma unroll 2
+#pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           uint32_t o[32], w[16];
           tmem_ld32(t_o + c * 32, o);

@@ -68,6 +68,30 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   return r;
 }
 
+// 2^a, 2^b by arithmetic on the FMA pipe, for a, b <= 64 (below -126 as at -126; NaN stays
+// NaN). n = round(x) through the addition of 1.5 * 2^23, f = x - n in [-0.5, 0.5], the
+// polynomial of degree 5 with the least relative error there (Remez exchange; 2.4e-7
+// with these fp32 coefficients), times 2^n built from n's bits.
+__device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-126.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-126.0f));
+  x = f2_pack(x0, x1);
+  const uint64_t t = f2_add(x, f2_pack(12582912.0f, 12582912.0f));
+  const uint64_t f = f2_fma(f2_add(t, f2_pack(-12582912.0f, -12582912.0f)), f2_pack(-1.0f, -1.0f), x);
+  uint64_t y = f2_fma(f2_pack(0.0013276472454890609f, 0.0013276472454890609f), f,
+                      f2_pack(0.009675540961325169f, 0.009675540961325169f));
+  y = f2_fma(y, f, f2_pack(0.05550713092088699f, 0.05550713092088699f));
+  y = f2_fma(y, f, f2_pack(0.24022120237350464f, 0.24022120237350464f));
+  y = f2_fma(y, f, f2_pack(0.6931469440460205f, 0.6931469440460205f));
+  y = f2_fma(y, f, f2_pack(1.0000001192092896f, 1.0000001192092896f));
+  float t0, t1;
+  f2_unpack(t, t0, t1);
+  const uint32_t e0 = (__float_as_uint(t0) << 23) + 0x3F800000u, e1 = (__float_as_uint(t1) << 23) + 0x3F800000u;
+  f2_unpack(f2_mul(y, f2_pack(__uint_as_float(e0), __uint_as_float(e1))), a, b);
+}
+
 // three-input maximum (sm_100); NaN operands are dropped, as by fmaxf
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;

@@ -44,6 +44,9 @@ constexpr int kOffBar = kOffRing + kRing * kTileBytes;
 constexpr int kSpSmem = kOffBar + 1024 + 1024;     // + barriers and notes + alignment
 constexpr unsigned kErrSpProd = 0x501, kErrSpMma = 0x502, kErrSpSoft = 0x503, kErrSpOut = 0x504, kErrSpDrain = 0x505;
 constexpr float kRescaleLog2 = 8.0f;
+// One pair of exponentials of kPolyOf is computed on the FMA pipe: the special-function
+// unit gives 16 a clock and SM, 1,024 clocks a tile, as long as the tile's products take.
+constexpr int kPolyOf = 4;
 
 struct SparseParams {
   const int32_t* blocks;  // [kv_heads, q_blocks, top_k]
@@ -534,10 +537,15 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
           const uint32_t* y = &x[e >> 4][2 * (e & 15)];
+          const uint64_t z = f2_fma(f2_pack(__uint_as_float(y[0]), __uint_as_float(y[1])), scale2, sub2);
           float a, b;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(y[0]), __uint_as_float(y[1])), scale2, sub2), a, b);
-          a = ex2_approx(a);
-          b = ex2_approx(b);
+          if (e % kPolyOf == kPolyOf - 1) {
+            exp2_poly2(z, a, b);
+          } else {
+            f2_unpack(z, a, b);
+            a = ex2_approx(a);
+            b = ex2_approx(b);
+          }
           sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, b));
           w[e] = E::pack(a, b);
         }
@@ -560,6 +568,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       tc_fence_after();
       i = 0;
       ++item;
+      if (m == -INFINITY) l = 0.0f;  // no key seen: exp2_poly2 gives 2^-126 for -inf
       if (p.parts > 1) {
         const int64_t at = ((int64_t)(it.head * p.q_blocks + it.q_block) * p.parts + it.part) * kQueryBlock + row_in;
         if (row < p.queries) p.ws_ml[at] = make_float2(m, l);

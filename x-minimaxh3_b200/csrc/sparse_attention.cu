@@ -46,7 +46,7 @@ constexpr unsigned kErrSpProd = 0x501, kErrSpMma = 0x502, kErrSpSoft = 0x503, kE
 constexpr float kRescaleLog2 = 8.0f;
 // One pair of exponentials of kPolyOf is computed on the FMA pipe: the special-function
 // unit gives 16 a clock and SM, 1,024 clocks a tile, as long as the tile's products take.
-constexpr int kPolyOf = 4;
+constexpr int kPolyOf = 8;
 
 struct SparseParams {
   const int32_t* blocks;  // [kv_heads, q_blocks, top_k]
@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
   uint64_t* p_full = s_full + 2;                                   // [2][2] a half of P is in TMEM, O is rescaled
   uint64_t* o_full = p_full + 4;                                   // [2] the item's O is complete
   uint64_t* turn = o_full + 2;                                     // [2] the stream's products of a tile are issued
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
+  uint64_t* h_done = turn + 2;                                     // [2] the product of P's first half is complete
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(h_done + 2);
   int* tiles_of = reinterpret_cast<int*>(tmem_slot + 1);           // [2] tiles of each stream
   int* empty_of = tiles_of + 2;                                    // [2] whether it has items without tiles
   ItemNote* item_note = reinterpret_cast<ItemNote*>(smem + kOffBar + 384);  // [2][kNotes] items that have tiles
@@ -199,6 +200,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&o_full[i], 1);
       mbar_init(&turn[i], 1);
+      mbar_init(&h_done[i], 1);
     }
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&kv_full[i], 2);  // one arrival per TMA warp
@@ -431,6 +433,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 #pragma unroll
           for (int k = 4 * h; k < 4 * h + 4; ++k)
             umma_f16_ts(t_o, t_s + k * 8, v_desc + ((k * 16 * 128) >> 4), kIdescO, !first || k > 0 ? 1u : 0u);
+          if (h == 0) umma_commit(&h_done[s]);
         }
         if (!ok) break;
         first = --left == 0;  // the next tile opens an item
@@ -488,77 +491,85 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         tmem_wait_st();
       }
-      // Two passes over the row, the second reading the scores again: TMEM is read in
-      // some 50 clocks, and short loops instead of 128 scores in registers keep the code
-      // small (unrolled, the warps waited for instructions).
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (i == 0) {  // the item's first maximum
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-      for (int c = 0; c < 2; ++c) {
-        uint32_t x[2][32];
-        tmem_ld32(t_s + c * 64, x[0]);
-        tmem_ld32(t_s + c * 64 + 32, x[1]);
-        tmem_wait_ld();
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          mx[0] = max3(mx[0], __uint_as_float(x[0][e]), __uint_as_float(x[0][e + 1]));
-          mx[1] = max3(mx[1], __uint_as_float(x[0][e + 2]), __uint_as_float(x[0][e + 3]));
-          mx[2] = max3(mx[2], __uint_as_float(x[1][e]), __uint_as_float(x[1][e + 1]));
-          mx[3] = max3(mx[3], __uint_as_float(x[1][e + 2]), __uint_as_float(x[1][e + 3]));
-        }
-      }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      const bool grow = (top - m) * p.scale_log2 > kRescaleLog2;  // also the first finite score (m = -inf)
-      if (i == 0) {
-        m = top;
-      } else if (__any_sync(0xFFFFFFFFu, grow)) {
-        const float f = grow ? ex2_approx((m - top) * p.scale_log2) : 1.0f;
-        if (grow) m = top;
-        l *= f;
-        // the product of the tile before is complete: its commit came before s_full's
-#pragma unroll 1
-        for (int c = 0; c < 8; ++c) {
-          uint32_t o[16];
-          tmem_ld16(t_o + c * 16, o);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t x[32];
+          tmem_ld32(t_s + c * 32, x);
           tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tmem_st16(t_o + c * 16, o);
+          for (int e = 0; e < 32; e += 8)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              mx[k] = max3(mx[k], __uint_as_float(x[e + 2 * k]), __uint_as_float(x[e + 2 * k + 1]));
         }
+        m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       }
-      const float sub = m == -INFINITY ? 0.0f : m * p.scale_log2;
-      const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(-sub, -sub);
-      uint64_t sum[2] = {0ull, 0ull};
+      // The weights of a half are computed with the maximum so far while its own maximum
+      // is found beside them; only where that is more than 2^8 higher (or the first finite
+      // score) are the sums so far rescaled and the half computed again.
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         uint32_t x[2][32], w[32];
         tmem_ld32(t_s + h * 64, x[0]);
         tmem_ld32(t_s + h * 64 + 32, x[1]);
         tmem_wait_ld();
+        uint64_t sum[2];
+#pragma unroll 1
+        for (;;) {
+          const float sub = m == -INFINITY ? 0.0f : m * p.scale_log2;
+          const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(-sub, -sub);
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          sum[0] = sum[1] = 0ull;
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const uint32_t* y = &x[e >> 4][2 * (e & 15)];
-          const uint64_t z = f2_fma(f2_pack(__uint_as_float(y[0]), __uint_as_float(y[1])), scale2, sub2);
-          float a, b;
-          if (e % kPolyOf == kPolyOf - 1) {
-            exp2_poly2(z, a, b);
-          } else {
-            f2_unpack(z, a, b);
-            a = ex2_approx(a);
-            b = ex2_approx(b);
+          for (int e = 0; e < 32; ++e) {
+            const float y0 = __uint_as_float(x[e >> 4][2 * (e & 15)]), y1 = __uint_as_float(x[e >> 4][2 * (e & 15) + 1]);
+            const uint64_t z = f2_fma(f2_pack(y0, y1), scale2, sub2);
+            float a, b;
+            if (e % kPolyOf == kPolyOf - 1) {
+              exp2_poly2(z, a, b);
+            } else {
+              f2_unpack(z, a, b);
+              a = ex2_approx(a);
+              b = ex2_approx(b);
+            }
+            mx[e & 3] = max3(mx[e & 3], y0, y1);
+            sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, b));
+            w[e] = E::pack(a, b);
           }
-          sum[e & 1] = f2_add(sum[e & 1], f2_pack(a, b));
-          w[e] = E::pack(a, b);
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          const bool grow = (top - m) * p.scale_log2 > kRescaleLog2;
+          if (!__any_sync(0xFFFFFFFFu, grow)) break;
+          const float f = grow ? ex2_approx((m - top) * p.scale_log2) : 1.0f;
+          if (grow) m = top;
+          l *= f;
+          // O holds what is complete: the tiles before (their commit came before s_full's)
+          // and, for the second half, the first half's product
+          if (h == 1) ok = mbar_wait(&h_done[s], t & 1, kErrSpSoft) && ok;
+          if (i > 0 || h == 1) {
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c * 16, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(t_o + c * 16, o);
+            }
+          }
         }
+        float s0, s1, s2, s3;
+        f2_unpack(sum[0], s0, s1);
+        f2_unpack(sum[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
         tmem_st32(t_s + h * 32, w);  // over columns already read
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[2 * s + h]);
       }
-      float s0, s1, s2, s3;
-      f2_unpack(sum[0], s0, s1);
-      f2_unpack(sum[1], s2, s3);
-      l += (s0 + s1) + (s2 + s3);
       if (++i < it.n) continue;
       // the item's last tile: its rows
       if (!mbar_wait(&o_full[s], item & 1, kErrSpOut)) {

@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(kMeanThreads, 6) block_means_kernel(const uint
 }
 static_assert(kMeanThreads == kHeadDim, "one thread per dim finishes a mean");
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 256, kSelThreadsMax = 512;
+constexpr int kSelPad = kHeadDim + 2;  // doubles per staged query row: conflict-free 16-byte reads
 constexpr int kSelRows = 8;  // query blocks per CTA: the M of one 64-bit matrix instruction; one warp each for the top-k
 
 // c[8 x 8] += a[8 x 4] b[4 x 8] in 64 bits
@@ -87,7 +88,7 @@ __device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
 // 64-bit key whose unsigned order is the order of the scores; 0 stands for "not to be
 // selected". NaN scores rank below every number.
 __device__ __forceinline__ unsigned long long score_key(double s) {
-  if (!(s == s)) return 1ull;
+  if (!(s == s)) return 1ull << 32;
   if (s == 0.0) s = 0.0;  // -0 and +0 are equal
   const unsigned long long b = (unsigned long long)__double_as_longlong(s);
   return (b >> 63) ? ~b : (b | 0x8000000000000000ull);  // -inf gives 0x000FF..F, above 1
@@ -100,9 +101,12 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 //
 // Scores: a warp takes 8 key blocks at a time, m8n8k4 in 64 bits. The contraction index
 // is permuted so that lane (g, t) reads 16 contiguous bytes of key block g (dims
-// 16 c + 4 t .. + 3) and uses them in four instructions; the 8 query rows stay in
-// registers in the same order.
-__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float* __restrict__ qm,
+// 16 c + 4 t .. + 3) and uses them in four instructions; the 8 query rows are read from
+// shared memory in the same order (in registers they would halve the CTAs per SM).
+//
+// Keys are kept as their high and low words: the high ones (20 bits of the mantissa)
+// nearly always decide alone.
+__global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const float* __restrict__ qm,
                                                                     const float* __restrict__ km, int64_t km_h,
                                                                     int64_t km_b, int group,
                                                                     int64_t q_blocks, int k_blocks, int top_k,
@@ -111,30 +115,32 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float*
                                                                     int32_t* __restrict__ out,
                                                                     int32_t* __restrict__ out_tiles) {
   extern __shared__ __align__(16) unsigned char sel_smem[];
-  double* qs = reinterpret_cast<double*>(sel_smem);                               // [rows][128]
-  unsigned long long* key = reinterpret_cast<unsigned long long*>(qs + kSelRows * kHeadDim);  // [rows][k_blocks]
+  double* qs = reinterpret_cast<double*>(sel_smem);                          // [kSelRows][kSelPad]
+  const int pitch = (k_blocks + 3) & ~3;
+  uint32_t* key_hi = reinterpret_cast<uint32_t*>(qs + kSelRows * kSelPad);   // [rows][pitch], 0 behind the last block
+  uint32_t* key_lo = key_hi + rows_per_cta * pitch;
   const int64_t tiles = (q_blocks + rows_per_cta - 1) / rows_per_cta;
   const int64_t kvh = blockIdx.x / tiles;
   const int64_t i0 = (blockIdx.x - kvh * tiles) * rows_per_cta;
   const int rows = (int)min((int64_t)rows_per_cta, q_blocks - i0);
-  for (int e = threadIdx.x; e < kSelRows * kHeadDim; e += kSelThreads) {
+  for (int e = threadIdx.x; e < kSelRows * kHeadDim; e += blockDim.x) {
     const int r = e / kHeadDim, d = e % kHeadDim;
     double s = 0.0;
     if (r < rows)
       for (int g = 0; g < group; ++g) s += (double)__ldg(qm + ((kvh * group + g) * q_blocks + i0 + r) * kHeadDim + d);
-    qs[e] = s;
+    qs[r * kSelPad + d] = s;
+  }
+  for (int e = threadIdx.x; e < rows * (pitch - k_blocks); e += blockDim.x) {
+    const int r = e / (pitch - k_blocks);
+    key_hi[r * pitch + k_blocks + e - r * (pitch - k_blocks)] = 0u;
   }
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   {
     const int g = lane >> 2, t = lane & 3;
-    double a[32];
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) a[4 * c + e] = qs[g * kHeadDim + 16 * c + 4 * t + e];
+    const double2* a = reinterpret_cast<const double2*>(qs + g * kSelPad + 4 * t);
     const float* base = km + kvh * km_h + 4 * t;
-    for (int j0 = warp * 8; j0 < k_blocks; j0 += kSelThreads / 32 * 8) {
+    for (int j0 = warp * 8; j0 < k_blocks; j0 += blockDim.x / 32 * 8) {
       float4 v[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -144,10 +150,11 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float*
       double s[2][2] = {{0.0, 0.0}, {0.0, 0.0}};  // two chains
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        mma_f64(s[0], a[4 * c], (double)v[c].x);
-        mma_f64(s[1], a[4 * c + 1], (double)v[c].y);
-        mma_f64(s[0], a[4 * c + 2], (double)v[c].z);
-        mma_f64(s[1], a[4 * c + 3], (double)v[c].w);
+        const double2 a0 = a[8 * c], a1 = a[8 * c + 1];
+        mma_f64(s[0], a0.x, (double)v[c].x);
+        mma_f64(s[1], a0.y, (double)v[c].y);
+        mma_f64(s[0], a1.x, (double)v[c].z);
+        mma_f64(s[1], a1.y, (double)v[c].w);
       }
       // lane (g, t): query block g, key blocks j0 + 2 t and j0 + 2 t + 1
 #pragma unroll
@@ -162,64 +169,78 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float*
           if (start + block > first) k = ~0ull;
           if (start > last) k = 0ull;
         }
-        key[(int64_t)g * k_blocks + j] = k;
+        key_hi[g * pitch + j] = (uint32_t)(k >> 32);
+        key_lo[g * pitch + j] = (uint32_t)k;
       }
     }
   }
   __syncthreads();
   if (warp >= rows) return;
-  const unsigned long long* mine = key + (int64_t)warp * k_blocks;
+  const uint32_t* hi = key_hi + warp * pitch;
+  const uint32_t* lo = key_lo + warp * pitch;
   int32_t* dst = out + (kvh * q_blocks + i0 + warp) * (int64_t)top_k;
-  // largest threshold with at least top_k keys at or above it; 1 (everything) when fewer exist
-  unsigned long long th = 0ull;
-  int above = k_blocks;  // keys >= th
-  bool enough = false;
-  // bits that all keys share need no search: th starts as their common prefix
-  unsigned long long hi = 0ull, lo = ~0ull;
-  for (int j = lane; j < k_blocks; j += 32) {
-    const unsigned long long k = mine[j];
-    hi = max(hi, k);
-    lo = min(lo, k);
-  }
-#pragma unroll
-  for (int i = 16; i > 0; i >>= 1) {
-    hi = max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, i));
-    lo = min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, i));
-  }
-  int top_bit = 63;
-  if (k_blocks > 0 && top_k <= k_blocks) {
-    top_bit = 63 - __clzll((long long)(hi ^ lo));  // -1: all equal
-    th = top_bit >= 63 ? 0ull : (hi >> (top_bit + 1)) << (top_bit + 1);
-    enough = th != 0ull;                           // every key is at or above the prefix
-  }
-  for (int bit = top_bit; bit >= 0; --bit) {
-    const unsigned long long c = th | (1ull << bit);
-    int n = 0;
-    for (int j = lane; j < k_blocks; j += 32) n += mine[j] >= c ? 1 : 0;
-    n = (int)__reduce_add_sync(0xFFFFFFFFu, (unsigned)n);
-    if (n >= top_k) {
-      th = c;
-      above = n;
-      enough = true;
-      if (n == top_k) break;  // exactly the selection: no lower bit changes it
+  // th: the largest high word with at least top_k keys at or above it (1 when fewer keys
+  // than that can be selected: a key of 0 cannot, and the high word of every other is not 0)
+  uint32_t th = 1u;
+  int above = 0;  // keys >= th
+  {
+    uint32_t most = 0u, least = ~0u;
+    for (int j = lane; j < k_blocks; j += 32) {
+      most = max(most, hi[j]);
+      least = min(least, hi[j]);
     }
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    least = __reduce_min_sync(0xFFFFFFFFu, least);
+    auto count = [&](uint32_t c) {  // keys with a high word >= c, c > 0
+      int n = 0;
+      for (int j = lane * 4; j < pitch; j += 128) {
+        const uint4 v = *reinterpret_cast<const uint4*>(hi + j);
+        n += (v.x >= c) + (v.y >= c) + (v.z >= c) + (v.w >= c);
+      }
+      return (int)__reduce_add_sync(0xFFFFFFFFu, (unsigned)n);
+    };
+    // bits that all keys share need no search
+    uint32_t c = 0u;
+    int bit = 31;
+    if (top_k <= k_blocks) {
+      bit = 31 - __clz((int)(most ^ least));  // -1: all equal
+      c = bit >= 31 ? 0u : (most >> (bit + 1)) << (bit + 1);
+    }
+    for (; bit >= 0; --bit) {
+      const int n = count(c | (1u << bit));
+      if (n >= top_k) {
+        c |= 1u << bit;
+        if (n == top_k) break;  // exactly the selection: no lower bit changes it
+      }
+    }
+    th = max(c, 1u);
+    above = count(th);
   }
-  if (!enough || th == 0ull) th = 1ull;
-  // keys above the threshold are all taken; of those equal to it the first ones
-  int equal_left = top_k;
-  if (enough && above > top_k) {
-    int n = 0;
-    for (int j = lane; j < k_blocks; j += 32) n += mine[j] > th ? 1 : 0;
-    equal_left = top_k - (int)__reduce_add_sync(0xFFFFFFFFu, (unsigned)n);
+  uint32_t th_lo = 0u;
+  int equal_left = top_k;  // keys equal to (th, th_lo) that are still to be taken, the first ones
+  if (above > top_k) {
+    auto count = [&](bool higher, uint32_t c) {  // keys above th, or equal to it with a low word >= c
+      int n = 0;
+      for (int j = lane; j < k_blocks; j += 32) n += hi[j] > th || (!higher && hi[j] == th && lo[j] >= c);
+      return (int)__reduce_add_sync(0xFFFFFFFFu, (unsigned)n);
+    };
+    for (int bit = 31; bit >= 0; --bit)
+      if (count(false, th_lo | (1u << bit)) >= top_k) th_lo |= 1u << bit;
+    equal_left = top_k - (th_lo == ~0u ? count(true, 0u) : count(false, th_lo + 1u));
   }
   int at = 0;
   for (int j0 = 0; j0 < k_blocks; j0 += 32) {
     const int j = j0 + lane;
-    const unsigned long long k = j < k_blocks ? mine[j] : 0ull;
+    const uint32_t h = j < k_blocks ? hi[j] : 0u;
     const unsigned lower = (1u << lane) - 1u;
-    const bool exact = above == top_k && enough;
-    const unsigned equal = __ballot_sync(0xFFFFFFFFu, !exact && k == th);
-    const bool take = k > th || (k == th && (exact || __popc(equal & lower) < equal_left));
+    bool take = h >= th, same = false;
+    if (above > top_k && h == th) {
+      const uint32_t l = lo[j];
+      take = l > th_lo;
+      same = l == th_lo;
+    }
+    const unsigned equal = __ballot_sync(0xFFFFFFFFu, same);
+    take = take || (same && __popc(equal & lower) < equal_left);
     const unsigned taken = __ballot_sync(0xFFFFFFFFu, take);
     if (take) dst[at + __popc(taken & lower)] = j;
     at += __popc(taken);
@@ -247,15 +268,15 @@ cudaError_t launch_block_means(const void* x, int64_t x_t, int64_t x_h, int64_t 
   return cudaGetLastError();
 }
 
-int64_t select_blocks_max() { return (200 * 1024 - kSelRows * kHeadDim * 8) / 8; }
+int64_t select_blocks_max() { return (200 * 1024 - kSelRows * kSelPad * 8) / 8 - 4; }
 
 cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream) {
   if (a.q_blocks <= 0 || a.kv_heads <= 0 || a.top_k <= 0) return cudaSuccess;
   if (a.k_blocks > select_blocks_max() || (reinterpret_cast<uintptr_t>(a.k_means) & 15) || a.km_h % 4 || a.km_b % 4)
     return cudaErrorNotSupported;
-  int rows = kSelRows;
-  while (rows > 1 && (int64_t)rows * a.k_blocks > select_blocks_max()) rows /= 2;
-  const int smem = (int)(kSelRows * kHeadDim * 8 + (int64_t)rows * a.k_blocks * 8);
+  int rows = (int)std::min<int64_t>(kSelRows, a.q_blocks);
+  while (rows > 1 && (int64_t)rows * (a.k_blocks + 4) > select_blocks_max()) rows = (rows + 1) / 2;
+  const int smem = (int)(kSelRows * kSelPad * 8 + (int64_t)rows * ((a.k_blocks + 3) / 4 * 4) * 8);
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -267,7 +288,9 @@ cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream)
   }
   const int64_t grid = a.kv_heads * ((a.q_blocks + rows - 1) / rows);
   if (grid > 0x7FFFFFFF) return cudaErrorNotSupported;
-  select_blocks_kernel<<<(unsigned)grid, kSelThreads, smem, stream>>>(
+  // few CTAs: more warps each, for the latency of their loads
+  const int threads = grid < num_sms(dev) ? kSelThreadsMax : kSelThreads;
+  select_blocks_kernel<<<(unsigned)grid, threads, smem, stream>>>(
       a.q_means, a.k_means, a.km_h, a.km_b, (int)(a.heads / a.kv_heads), a.q_blocks, (int)a.k_blocks, (int)a.top_k, rows, (int)a.block,
       a.queries, a.keys, a.causal ? 1 : 0, a.out, a.tiles);
   return cudaGetLastError();

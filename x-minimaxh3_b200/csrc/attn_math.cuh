@@ -6,7 +6,35 @@
 
 #include "common.cuh"
 
+#include <utility>
+
 namespace h3 {
+
+// Dependent launches: the kernels of one operator follow one another on a stream. The next
+// one may start its CTAs once all of this one's have called launch_next(), and reads what
+// this one writes only behind wait_previous(), which waits for its end. Every kernel of a
+// chain waits before it writes anything, so nothing of it overlaps the kernel before.
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// kernel<<<grid, block, smem, stream>>>(args...), after_previous: as a dependent of the launch before it
+template <typename... P, typename... A>
+cudaError_t launch_chained(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                           bool after_previous, A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  if (after_previous) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<A>(args)...);
+}
 
 constexpr int kHeadDim = 128;  // the head dim of every attention kernel of this library
 

@@ -26,22 +26,33 @@ namespace {
 constexpr int kMeanThreads = 128;  // 8 half-warps, one block row each at a time
 constexpr int kMeanUnroll = 8;     // rows in flight per half-warp
 
-// One CTA per (block, head). A half-warp reads a 256-byte row as 16 lanes x 16 bytes.
+struct MeanSource {
+  const uint16_t* x;
+  int64_t x_t, x_h, tokens, blocks;
+  int heads, block;
+  float* means;
+};
+
+// One CTA per (block, head) of two tensors (the second may be empty). A half-warp reads
+// a 256-byte row as 16 lanes x 16 bytes.
 // HBM-bound in principle; the loads of a 64-key block are few, so what counts is how
 // many small CTAs an SM holds. Consecutive CTAs take consecutive heads of the same tokens.
 template <bool F16>
-__global__ void __launch_bounds__(kMeanThreads, 6) block_means_kernel(const uint16_t* __restrict__ x, int64_t x_t,
-                                                                   int64_t x_h, int64_t tokens, int heads, int block,
-                                                                   int64_t blocks, float* __restrict__ means) {
+__global__ void __launch_bounds__(kMeanThreads, 6) block_means_kernel(const MeanSource first, const MeanSource second) {
   using E = Elem16<F16>;
   __shared__ double part[kMeanThreads / 32][kHeadDim];
+  launch_next();
   const int hw = threadIdx.x >> 4, l = threadIdx.x & 15, warp = threadIdx.x >> 5;
-  const int64_t b = blockIdx.x / heads;
-  const int h = (int)(blockIdx.x - b * heads);
-  const int64_t t0 = b * block;
-  const int rows = (int)min((int64_t)block, tokens - t0);
+  const int64_t ctas = first.blocks * first.heads;
+  const bool of_first = (int64_t)blockIdx.x < ctas;
+  const MeanSource& src_of = of_first ? first : second;
+  const int64_t cta = of_first ? blockIdx.x : blockIdx.x - ctas;
+  const int64_t b = cta / src_of.heads;
+  const int h = (int)(cta - b * src_of.heads);
+  const int64_t t0 = b * src_of.block, x_t = src_of.x_t;
+  const int rows = (int)min((int64_t)src_of.block, src_of.tokens - t0);
   double s[8] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0, 0.0};
-  const uint16_t* src = x + h * x_h + t0 * x_t + l * 8;
+  const uint16_t* src = src_of.x + h * src_of.x_h + t0 * x_t + l * 8;
   for (int r0 = hw; r0 < rows; r0 += kMeanThreads / 16 * kMeanUnroll) {
     uint4 v[kMeanUnroll];
 #pragma unroll
@@ -70,7 +81,7 @@ __global__ void __launch_bounds__(kMeanThreads, 6) block_means_kernel(const uint
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < kMeanThreads / 32; ++i) sum += part[i][threadIdx.x];
-  means[((int64_t)h * blocks + b) * kHeadDim + threadIdx.x] = (float)(sum / (double)rows);
+  src_of.means[((int64_t)h * src_of.blocks + b) * kHeadDim + threadIdx.x] = (float)(sum / (double)rows);
 }
 static_assert(kMeanThreads == kHeadDim, "one thread per dim finishes a mean");
 
@@ -106,19 +117,23 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 //
 // Keys are kept as their high and low words: the high ones (20 bits of the mantissa)
 // nearly always decide alone.
-__global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const float* __restrict__ qm,
-                                                                    const float* __restrict__ km, int64_t km_h,
+__global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const float* qm,
+                                                                    const float* km, int64_t km_h,
                                                                     int64_t km_b, int group,
                                                                     int64_t q_blocks, int k_blocks, int top_k,
                                                                     int rows_per_cta, int block, int64_t queries,
                                                                     int64_t keys, int causal,
                                                                     int32_t* __restrict__ out,
-                                                                    int32_t* __restrict__ out_tiles) {
+                                                                    int32_t* __restrict__ out_tiles,
+                                                                    const uint16_t* __restrict__ q_row,
+                                                                    int64_t q_row_h, int q_row_f16) {
   extern __shared__ __align__(16) unsigned char sel_smem[];
   double* qs = reinterpret_cast<double*>(sel_smem);                          // [kSelRows][kSelPad]
   const int pitch = (k_blocks + 3) & ~3;
   uint32_t* key_hi = reinterpret_cast<uint32_t*>(qs + kSelRows * kSelPad);   // [rows][pitch], 0 behind the last block
   uint32_t* key_lo = key_hi + rows_per_cta * pitch;
+  launch_next();
+  wait_previous();
   const int64_t tiles = (q_blocks + rows_per_cta - 1) / rows_per_cta;
   const int64_t kvh = blockIdx.x / tiles;
   const int64_t i0 = (blockIdx.x - kvh * tiles) * rows_per_cta;
@@ -126,8 +141,16 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
   for (int e = threadIdx.x; e < kSelRows * kHeadDim; e += blockDim.x) {
     const int r = e / kHeadDim, d = e % kHeadDim;
     double s = 0.0;
-    if (r < rows)
-      for (int g = 0; g < group; ++g) s += (double)__ldg(qm + ((kvh * group + g) * q_blocks + i0 + r) * kHeadDim + d);
+    if (r < rows) {
+      for (int g = 0; g < group; ++g) {
+        if (q_row != nullptr) {  // one query: it is its own mean
+          const uint32_t w = __ldg(q_row + (kvh * group + g) * q_row_h + d);
+          s += (double)(q_row_f16 ? Elem16<true>::lo(w) : Elem16<false>::lo(w));
+        } else {
+          s += (double)*(qm + ((kvh * group + g) * q_blocks + i0 + r) * kHeadDim + d);
+        }
+      }
+    }
     qs[r * kSelPad + d] = s;
   }
   for (int e = threadIdx.x; e < rows * (pitch - k_blocks); e += blockDim.x) {
@@ -145,7 +168,7 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (j0 + g < k_blocks) v[c] = __ldg(reinterpret_cast<const float4*>(base + (j0 + g) * km_b + 16 * c));
+        if (j0 + g < k_blocks) v[c] = *reinterpret_cast<const float4*>(base + (j0 + g) * km_b + 16 * c);
       }
       double s[2][2] = {{0.0, 0.0}, {0.0, 0.0}};  // two chains
 #pragma unroll
@@ -252,20 +275,24 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
 
 }  // namespace
 
-cudaError_t launch_block_means(const void* x, int64_t x_t, int64_t x_h, int64_t tokens, int64_t heads, int64_t block,
-                               bool f16, float* means, cudaStream_t stream) {
-  const int64_t blocks = (tokens + block - 1) / block;
-  if (blocks * heads == 0) return cudaSuccess;
-  if ((reinterpret_cast<uintptr_t>(x) & 15) || x_t % 8 || x_h % 8 || blocks * heads > 0x7FFFFFFF)
-    return cudaErrorNotSupported;
-  const unsigned grid = (unsigned)(blocks * heads);
-  if (f16)
-    block_means_kernel<true><<<grid, kMeanThreads, 0, stream>>>(static_cast<const uint16_t*>(x), x_t, x_h, tokens,
-                                                                (int)heads, (int)block, blocks, means);
-  else
-    block_means_kernel<false><<<grid, kMeanThreads, 0, stream>>>(static_cast<const uint16_t*>(x), x_t, x_h, tokens,
-                                                                 (int)heads, (int)block, blocks, means);
-  return cudaGetLastError();
+cudaError_t launch_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b, bool f16, cudaStream_t stream) {
+  MeanSource src[2];
+  int64_t ctas = 0;
+  for (int i = 0; i < 2; ++i) {
+    const BlockMeansArgs& m = i ? b : a;
+    src[i].x = static_cast<const uint16_t*>(m.x);
+    src[i].x_t = m.x_t; src[i].x_h = m.x_h; src[i].tokens = m.tokens;
+    src[i].heads = (int)m.heads; src[i].block = (int)m.block;
+    src[i].blocks = m.tokens > 0 && m.heads > 0 ? (m.tokens + m.block - 1) / m.block : 0;
+    src[i].means = m.means;
+    ctas += src[i].blocks * m.heads;
+    if (src[i].blocks > 0 && ((reinterpret_cast<uintptr_t>(m.x) & 15) || m.x_t % 8 || m.x_h % 8))
+      return cudaErrorNotSupported;
+  }
+  if (ctas == 0) return cudaSuccess;
+  if (ctas > 0x7FFFFFFF) return cudaErrorNotSupported;
+  return launch_chained(f16 ? block_means_kernel<true> : block_means_kernel<false>, (unsigned)ctas, kMeanThreads, 0,
+                        stream, false, src[0], src[1]);
 }
 
 int64_t select_blocks_max() { return (200 * 1024 - kSelRows * kSelPad * 8) / 8 - 4; }
@@ -290,10 +317,10 @@ cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream)
   if (grid > 0x7FFFFFFF) return cudaErrorNotSupported;
   // few CTAs: more warps each, for the latency of their loads
   const int threads = grid < num_sms(dev) ? kSelThreadsMax : kSelThreads;
-  select_blocks_kernel<<<(unsigned)grid, threads, smem, stream>>>(
-      a.q_means, a.k_means, a.km_h, a.km_b, (int)(a.heads / a.kv_heads), a.q_blocks, (int)a.k_blocks, (int)a.top_k, rows, (int)a.block,
-      a.queries, a.keys, a.causal ? 1 : 0, a.out, a.tiles);
-  return cudaGetLastError();
+  return launch_chained(select_blocks_kernel, (unsigned)grid, threads, smem, stream, a.chained, a.q_means, a.k_means,
+                        a.km_h, a.km_b, (int)(a.heads / a.kv_heads), a.q_blocks, (int)a.k_blocks, (int)a.top_k, rows,
+                        (int)a.block, a.queries, a.keys, a.causal ? 1 : 0, a.out, a.tiles,
+                        static_cast<const uint16_t*>(a.q_row), a.q_row_h, a.q_row_f16 ? 1 : 0);
 }
 
 }  // namespace h3

@@ -1526,23 +1526,19 @@ int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t x_sh, int6
   if (tokens < 0 || heads < 0 || block <= 0 || block > (1 << 20)) return fail(H3B200_ERR_INVALID, "%s: bad shape", who);
   if (tokens == 0 || heads == 0) return H3B200_OK;
   if (!x || !means) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
-  return from_cuda(h3::launch_block_means(x, x_st, x_sh, tokens, heads, block, dtype == H3B200_DTYPE_F16, means, S(stream)), who);
+  h3::BlockMeansArgs a;
+  a.x = x; a.x_t = x_st; a.x_h = x_sh; a.tokens = tokens; a.heads = heads; a.block = block; a.means = means;
+  return from_cuda(h3::launch_block_means(a, h3::BlockMeansArgs(), dtype == H3B200_DTYPE_F16, S(stream)), who);
 }
 
-static int select_impl(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb, int64_t heads,
-                       int64_t kv_heads, int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
-                       int32_t* blocks, int32_t* tiles, h3b200_stream_t stream, const char* who) {
-  if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
-  if (queries < 0 || keys < 0 || block <= 0 || block > (1 << 20) || top_k <= 0 || top_k > (1 << 24)) return fail(H3B200_ERR_INVALID, "%s: bad shape (top_k and block must be positive)", who);
-  if (queries == 0) return H3B200_OK;
-  const int64_t k_blocks = (keys + block - 1) / block;
-  if (k_blocks > h3::select_blocks_max()) return fail(H3B200_ERR_UNSUPPORTED, "%s: %lld key blocks, at most %lld are built", who, (long long)k_blocks, (long long)h3::select_blocks_max());
-  if (!q_means || (keys > 0 && !k_means) || !blocks) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
-  h3::SelectBlocksArgs a;
-  a.q_means = q_means; a.k_means = k_means; a.km_h = km_sh; a.km_b = km_sb; a.heads = heads; a.kv_heads = kv_heads;
-  a.q_blocks = (queries + h3::kQueryBlock - 1) / h3::kQueryBlock;
-  a.k_blocks = k_blocks; a.top_k = top_k; a.block = block; a.queries = queries; a.keys = keys;
-  a.causal = causal != 0; a.out = blocks; a.tiles = tiles;
+static int select_impl(h3::SelectBlocksArgs& a, h3b200_stream_t stream, const char* who) {
+  if (const int rc = attn_heads(a.heads, a.kv_heads, who)) return rc;
+  if (a.queries < 0 || a.keys < 0 || a.block <= 0 || a.block > (1 << 20) || a.top_k <= 0 || a.top_k > (1 << 24)) return fail(H3B200_ERR_INVALID, "%s: bad shape (top_k and block must be positive)", who);
+  if (a.queries == 0) return H3B200_OK;
+  a.q_blocks = (a.queries + h3::kQueryBlock - 1) / h3::kQueryBlock;
+  a.k_blocks = (a.keys + a.block - 1) / a.block;
+  if (a.k_blocks > h3::select_blocks_max()) return fail(H3B200_ERR_UNSUPPORTED, "%s: %lld key blocks, at most %lld are built", who, (long long)a.k_blocks, (long long)h3::select_blocks_max());
+  if ((!a.q_means && !a.q_row) || (a.keys > 0 && !a.k_means) || !a.out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
   return from_cuda(h3::launch_select_blocks(a, S(stream)), who);
 }
 
@@ -1550,7 +1546,11 @@ int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t
                              int64_t kv_heads, int64_t queries, int64_t keys, int64_t block, int64_t top_k, int causal,
                              int32_t* blocks, h3b200_stream_t stream) {
   H3_GUARD("select_key_blocks", stream);
-  return select_impl(q_means, k_means, km_sh, km_sb, heads, kv_heads, queries, keys, block, top_k, causal, blocks, nullptr, stream, "select_key_blocks");
+  h3::SelectBlocksArgs a;
+  a.q_means = q_means; a.k_means = k_means; a.km_h = km_sh; a.km_b = km_sb;
+  a.heads = heads; a.kv_heads = kv_heads; a.queries = queries; a.keys = keys; a.block = block; a.top_k = top_k;
+  a.causal = causal != 0; a.out = blocks;
+  return select_impl(a, stream, "select_key_blocks");
 }
 
 int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k,
@@ -1560,13 +1560,14 @@ int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int6
   return h3::block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block, current_sms());
 }
 
-// tiles: h3::list_tiles of each list where the caller knows them, else nullptr
+// tiles: h3::list_tiles of each list where the caller knows them, else nullptr; chained: the
+// launch before on this stream was the selection
 static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
                              const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks, const int32_t* tiles,
                              int64_t top_k, int64_t block, void* out, int64_t o_st, int64_t o_sh, float* lse,
                              int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys, int64_t heads,
                              int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
-                             int64_t workspace_bytes, h3b200_stream_t stream, const char* who) {
+                             int64_t workspace_bytes, bool chained, h3b200_stream_t stream, const char* who) {
   if (const int rc = attn_dtype(dtype, who)) return rc;
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
   if (queries < 0 || keys <= 0 || top_k <= 0) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys and top_k must be positive)", who);
@@ -1589,7 +1590,7 @@ static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const vo
     a.pages = (keys + block - 1) / block; a.page_size = block; a.rows = keys;
     a.out = out; a.o_b = 0; a.o_h = o_sh; a.lse = lse; a.l_b = 0; a.l_h = l_sh;
     a.batch = 1; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale;
-    a.workspace = workspace; a.f16 = dtype == H3B200_DTYPE_F16;
+    a.workspace = workspace; a.f16 = dtype == H3B200_DTYPE_F16; a.chained = chained;
     return from_cuda(h3::launch_paged_decode(a, S(stream)), who);
   }
   h3::SparseAttnArgs a;
@@ -1599,7 +1600,7 @@ static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const vo
   a.queries = queries; a.keys = keys; a.heads = heads; a.kv_heads = kv_heads; a.top_k = top_k; a.block = block;
   a.scale = scale; a.causal = causal != 0;
   a.out = out; a.o_t = o_st; a.o_h = o_sh; a.lse = lse; a.l_t = l_st; a.l_h = l_sh;
-  a.f16 = dtype == H3B200_DTYPE_F16;
+  a.f16 = dtype == H3B200_DTYPE_F16; a.chained = chained;
   return from_cuda(h3::launch_block_sparse_attention(a, S(stream)), who);
 }
 
@@ -1611,7 +1612,7 @@ int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, con
                                   int64_t workspace_bytes, h3b200_stream_t stream) {
   H3_GUARD("block_sparse_attention", stream);
   return block_sparse_impl(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, nullptr, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
-                           heads, kv_heads, scale, causal, dtype, workspace, workspace_bytes, stream, "block_sparse_attention");
+                           heads, kv_heads, scale, causal, dtype, workspace, workspace_bytes, false, stream, "block_sparse_attention");
 }
 
 int64_t h3b200_sparse_attention_workspace_bytes(int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
@@ -1641,18 +1642,34 @@ int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const voi
   uint8_t* base = static_cast<uint8_t*>(workspace);
   float* qm = reinterpret_cast<float*>(base);
   base += round_up(heads * ((queries + h3::kQueryBlock - 1) / h3::kQueryBlock) * row, 256);
-  if (const int rc = h3b200_attention_block_means(q, q_st, q_sh, queries, heads, h3::kQueryBlock, dtype, qm, stream)) return rc;
+  if (const int rc = attn_dtype(dtype, who)) return rc;
+  if (!q || !k || !v || !blocks || !out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
+  const bool f16 = dtype == H3B200_DTYPE_F16;
+  h3::SelectBlocksArgs sel;
+  h3::BlockMeansArgs mq, mk;
+  if (queries == 1) {  // one query is its own mean
+    sel.q_row = q; sel.q_row_h = q_sh; sel.q_row_f16 = f16;
+  } else {
+    mq.x = q; mq.x_t = q_st; mq.x_h = q_sh; mq.tokens = queries; mq.heads = heads; mq.block = h3::kQueryBlock; mq.means = qm;
+    sel.q_means = qm;
+  }
   if (k_means == nullptr) {
     float* km = reinterpret_cast<float*>(base);
     base += round_up(kv_heads * k_blocks * row, 256);
-    if (const int rc = h3b200_attention_block_means(k, k_st, k_sh, keys, kv_heads, block, dtype, km, stream)) return rc;
+    mk.x = k; mk.x_t = k_st; mk.x_h = k_sh; mk.tokens = keys; mk.heads = kv_heads; mk.block = block; mk.means = km;
     k_means = km; km_sh = k_blocks * h3::kHeadDim; km_sb = h3::kHeadDim;
   }
+  if (const int rc = from_cuda(h3::launch_block_means(mq, mk, f16, S(stream)), who)) return rc;
+  sel.k_means = k_means; sel.km_h = km_sh; sel.km_b = km_sb;
+  sel.heads = heads; sel.kv_heads = kv_heads; sel.queries = queries; sel.keys = keys; sel.block = block; sel.top_k = top_k;
+  sel.causal = causal != 0; sel.out = blocks;
   // the lists' tile counts go where the attention would count them
   int32_t* tiles = queries > 1 ? reinterpret_cast<int32_t*>(base) : nullptr;
-  if (const int rc = select_impl(qm, k_means, km_sh, km_sb, heads, kv_heads, queries, keys, block, top_k, causal, blocks, tiles, stream, who)) return rc;
+  sel.tiles = tiles;
+  sel.chained = mq.tokens > 0 || mk.tokens > 0;
+  if (const int rc = select_impl(sel, stream, who)) return rc;
   return block_sparse_impl(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, tiles, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
-                           heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, stream, who);
+                           heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, true, stream, who);
 }
 
 }  // extern "C"

@@ -332,6 +332,7 @@ struct PagedDecodeArgs {
   float scale = 0.0f;
   void* workspace = nullptr;  // paged_decode_workspace_bytes, 16-byte aligned
   bool f16 = false;
+  bool chained = false;  // as a dependent of the launch before it (block selection)
 };
 int64_t paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms);
 cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream);
@@ -339,8 +340,13 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream);
 constexpr int kQueryBlock = 128;  // query rows that share a selection of key blocks
 
 // fp32 [heads, ceil(tokens / block), 128] means of the blocks of x [tokens, heads, 128] (block_select.cu)
-cudaError_t launch_block_means(const void* x, int64_t x_t, int64_t x_h, int64_t tokens, int64_t heads, int64_t block,
-                               bool f16, float* means, cudaStream_t stream);
+// of two tensors in one launch (the second may have no tokens)
+struct BlockMeansArgs {
+  const void* x = nullptr;
+  int64_t x_t = 0, x_h = 0, tokens = 0, heads = 0, block = 1;
+  float* means = nullptr;
+};
+cudaError_t launch_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b, bool f16, cudaStream_t stream);
 // out [kv_heads, q_blocks, top_k]: selected key blocks, ascending, -1 behind them
 struct SelectBlocksArgs {
   const float *q_means = nullptr, *k_means = nullptr;  // q contiguous, k rows at strides
@@ -349,6 +355,11 @@ struct SelectBlocksArgs {
   bool causal = false;
   int32_t* out = nullptr;
   int32_t* tiles = nullptr;  // optional [kv_heads, q_blocks]: list_tiles of each list
+  // one query: its rows [heads, 128] (16-bit, head stride q_row_h) in place of q_means
+  const void* q_row = nullptr;
+  int64_t q_row_h = 0;
+  bool q_row_f16 = false;
+  bool chained = false;      // as a dependent of the launch before it (block means)
 };
 // 128-key tiles of a list of `count` blocks
 __host__ __device__ inline int list_tiles(int count, int subs_per_block) { return (count * subs_per_block + 1) / 2; }
@@ -370,6 +381,7 @@ struct SparseAttnArgs {
   const int32_t* tiles = nullptr;  // list_tiles of each list, where the caller knows them
   void* workspace = nullptr;       // block_sparse_workspace_bytes, 16-byte aligned
   bool f16 = false;
+  bool chained = false;            // as a dependent of the launch before it (block selection)
 };
 int64_t block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k, int64_t block,
                                      int sms);

@@ -81,6 +81,8 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
   constexpr int R = 8 * NT;
   __shared__ float sm_acc[kDecWarps][R][kHeadDim];
   __shared__ float sm_m[kDecWarps][R], sm_l[kDecWarps][R];
+  launch_next();
+  wait_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int64_t item = blockIdx.x / p.splits;
   const int split = (int)(blockIdx.x - item * p.splits);
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
   const uint16_t* vb = p.v + kvh * p.v_head;
 
   // page ids of the two 8-key halves of a step (page sizes are multiples of 8), -1: no keys
-  auto lookup = [&](int j) { return j < end ? __ldg(table + j / p.page_size) : -1; };
+  auto lookup = [&](int j) { return j < end ? table[j / p.page_size] : -1; };
   int id0 = lookup(begin + warp * 16), id1 = lookup(begin + warp * 16 + 8);
   for (int j = begin + warp * 16; j < end; j += kDecWarps * 16) {
     const int pid[2] = {id0, id1};
@@ -271,30 +273,36 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
   }
 }
 
-// One warp per (sequence, head): out = sum_s exp(m_s - m) O_s / sum_s exp(m_s - m) l_s.
-template <bool F16>
-__global__ void __launch_bounds__(128) decode_join_kernel(const DecodeParams p, int64_t total, int row_tile) {
+// out = sum_s exp(m_s - m) O_s / sum_s exp(m_s - m) l_s of one (sequence, head) by W warps:
+// warp w adds the splits w, w + W, ..., then the warps' sums are added in their order.
+// One warp is enough for a few splits; a hundred of them (one long sequence) would be
+// a chain of L2 latencies.
+template <bool F16, int W>
+__global__ void __launch_bounds__(256) decode_join_kernel(const DecodeParams p, int64_t total, int row_tile) {
   using E = Elem16<F16>;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= total) return;
-  const int lane = threadIdx.x & 31;
-  const int b = (int)(row / p.heads), head = (int)(row % p.heads);
+  constexpr int kRows = 8 / W;
+  __shared__ float4 sm_o[8][32];
+  __shared__ float sm_sum[8], sm_max[8];
+  wait_previous();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, w = warp % W;
+  const int64_t row = (int64_t)blockIdx.x * kRows + warp / W;
+  const bool live = row < total;
+  const int b = live ? (int)(row / p.heads) : 0, head = live ? (int)(row % p.heads) : 0;
   const int kvh = head / p.group, in_group = head % p.group;
   const int64_t item = ((int64_t)b * p.kv_heads + kvh) * p.row_tiles + in_group / row_tile;
-  const int r = in_group % row_tile;
   int begin, end;
-  const int parts = split_range(sequence_length(p, b), p.splits, p.part_min, 0, begin, end);
-  const int64_t at = item * p.splits * row_tile + r;
+  const int parts = live ? split_range(sequence_length(p, b), p.splits, p.part_min, 0, begin, end) : 0;
+  const int64_t at = item * p.splits * row_tile + in_group % row_tile;
   float mx = -INFINITY;
-  for (int s = lane; s < parts; s += 32) mx = fmaxf(mx, __ldcg(&p.ws_ml[at + (int64_t)s * row_tile].x));
+  for (int s = w + W * lane; s < parts; s += W * 32) mx = fmaxf(mx, p.ws_ml[at + (int64_t)s * row_tile].x);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, i));
   float sum = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = __ldcg(&p.ws_ml[at + (int64_t)s * row_tile]);
-    const float4 a = __ldcg(reinterpret_cast<const float4*>(p.ws_acc + (at + (int64_t)s * row_tile) * kHeadDim) + lane);
+  for (int s = w; s < parts; s += W) {
+    const float2 ml = p.ws_ml[at + (int64_t)s * row_tile];
+    const float4 a = *(reinterpret_cast<const float4*>(p.ws_acc + (at + (int64_t)s * row_tile) * kHeadDim) + lane);
     const float f = mx == -INFINITY ? 0.0f : exp2f((ml.x - mx) * p.scale_log2);
     sum = fmaf(ml.y, f, sum);
     o.x = fmaf(a.x, f, o.x);
@@ -302,6 +310,32 @@ __global__ void __launch_bounds__(128) decode_join_kernel(const DecodeParams p, 
     o.z = fmaf(a.z, f, o.z);
     o.w = fmaf(a.w, f, o.w);
   }
+  if constexpr (W > 1) {
+    sm_o[warp][lane] = o;
+    if (lane == 0) {
+      sm_sum[warp] = sum;
+      sm_max[warp] = mx;
+    }
+    __syncthreads();
+    if (w != 0) return;
+    float all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < W; ++i) all = fmaxf(all, sm_max[warp + i]);
+    sum = 0.0f;
+    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float f = all == -INFINITY ? 0.0f : exp2f((sm_max[warp + i] - all) * p.scale_log2);
+      const float4 a = sm_o[warp + i][lane];
+      sum = fmaf(sm_sum[warp + i], f, sum);
+      o.x = fmaf(a.x, f, o.x);
+      o.y = fmaf(a.y, f, o.y);
+      o.z = fmaf(a.z, f, o.z);
+      o.w = fmaf(a.w, f, o.w);
+    }
+    mx = all;
+  }
+  if (!live) return;
   const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
   uint2 y;
   y.x = E::pack(o.x * inv, o.y * inv);
@@ -314,7 +348,8 @@ __global__ void __launch_bounds__(128) decode_join_kernel(const DecodeParams p, 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 constexpr int kPartMin = 64;     // keys: one 16-key step of each warp
-constexpr int kMaxSplits = 256;
+constexpr int kPartGood = 512;   // keys whose reading outweighs a part's own cost by far
+constexpr int kMaxSplits = 512;
 
 int row_tile_of(int64_t group) { return group <= 8 ? 8 : 16; }
 
@@ -323,9 +358,13 @@ int row_tile_of(int64_t group) { return group <= 8 ? 8 : 16; }
 int paged_decode_splits(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms) {
   const int64_t group = heads / kv_heads;
   const int64_t items = batch * kv_heads * ((group + row_tile_of(group) - 1) / row_tile_of(group));
+  const int64_t slots = (int64_t)sms * (row_tile_of(group) == 8 ? 3 : 2);  // CTAs the GPU holds at once
+  // Few items: as many parts as fit at once (a part more would wait for a whole one), down
+  // to one step per warp. Many items, of lengths only the GPU knows: parts short enough
+  // that the last ones to finish are a small part of the work.
   const int64_t most = std::max<int64_t>(1, (max_keys + kPartMin - 1) / kPartMin);
-  const int64_t want = (4ll * sms + items - 1) / items;
-  return (int)std::min<int64_t>(kMaxSplits, std::min(most, want));
+  const int64_t good = std::min<int64_t>(8, std::max<int64_t>(1, max_keys / kPartGood));
+  return (int)std::min<int64_t>(kMaxSplits, std::min(most, std::max<int64_t>(slots / items, good)));
 }
 
 int64_t paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms) {
@@ -364,20 +403,16 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream) {
   p.ws_acc = static_cast<float*>(a.workspace);
   p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + items * p.splits * tile * kHeadDim);
   const unsigned grid = (unsigned)(items * p.splits);
-  if (a.f16) {
-    if (tile == 8) paged_decode_kernel<true, 1><<<grid, kDecThreads, 0, stream>>>(p);
-    else paged_decode_kernel<true, 2><<<grid, kDecThreads, 0, stream>>>(p);
-  } else {
-    if (tile == 8) paged_decode_kernel<false, 1><<<grid, kDecThreads, 0, stream>>>(p);
-    else paged_decode_kernel<false, 2><<<grid, kDecThreads, 0, stream>>>(p);
-  }
-  cudaError_t e = cudaGetLastError();
+  auto kernel = a.f16 ? (tile == 8 ? paged_decode_kernel<true, 1> : paged_decode_kernel<true, 2>)
+                      : (tile == 8 ? paged_decode_kernel<false, 1> : paged_decode_kernel<false, 2>);
+  const cudaError_t e = launch_chained(kernel, grid, kDecThreads, 0, stream, a.chained, p);
   if (e != cudaSuccess || p.splits == 1) return e;
   const int64_t total = a.batch * a.heads;
-  const unsigned jgrid = (unsigned)((total + 3) / 4);
-  if (a.f16) decode_join_kernel<true><<<jgrid, 128, 0, stream>>>(p, total, tile);
-  else decode_join_kernel<false><<<jgrid, 128, 0, stream>>>(p, total, tile);
-  return cudaGetLastError();
+  if (p.splits > 8)
+    return launch_chained(a.f16 ? decode_join_kernel<true, 8> : decode_join_kernel<false, 8>, (unsigned)total, 256, 0,
+                          stream, true, p, total, tile);
+  return launch_chained(a.f16 ? decode_join_kernel<true, 1> : decode_join_kernel<false, 1>, (unsigned)((total + 7) / 8),
+                        256, 0, stream, true, p, total, tile);
 }
 
 }  // namespace h3

@@ -117,7 +117,7 @@ __device__ __forceinline__ int sub_key(const SparseParams& p, const int32_t* lis
   const int per = p.block / kSubKeys;
   const int e = sub / per;
   if (e >= p.top_k) return -1;
-  const int id = __ldg(list + e);
+  const int id = list[e];
   if (id < 0 || id >= p.k_blocks) return -1;
   return id * p.block + (sub - e * per) * kSubKeys;
 }
@@ -154,7 +154,7 @@ __device__ __forceinline__ Work work_of(const SparseParams& p, int idx) {
   if (p.causal) w.q_block = p.q_blocks - 1 - w.q_block;  // the longest lists first
   const int at = (w.head / p.group) * p.q_blocks + w.q_block;
   w.list = p.blocks + (int64_t)at * p.top_k;
-  const int total = __ldg(p.tiles + at);
+  const int total = p.tiles[at];
   const int per = (total + p.parts - 1) / p.parts;
   w.first = min(total, w.part * per);
   w.n = min(total - w.first, per);
@@ -212,6 +212,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
   }
+  launch_next();
+  wait_previous();  // lists and tile counts
   if (warp == 8 || warp == 9) {
     const int s = warp - 8;
     int tiles = 0;
@@ -649,6 +651,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 // tiles[row] of each list: up to its last block that exists
 __global__ void __launch_bounds__(128) count_tiles_kernel(const int32_t* blocks, int64_t rows, int top_k, int k_blocks,
                                                           int subs_per_block, int32_t* tiles) {
+  launch_next();
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int lane = threadIdx.x & 31;
@@ -665,6 +668,7 @@ __global__ void __launch_bounds__(128) count_tiles_kernel(const int32_t* blocks,
 template <bool F16>
 __global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) {
   using E = Elem16<F16>;
+  wait_previous();
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (at >= (int64_t)p.heads * p.queries) return;
   const int lane = threadIdx.x & 31;
@@ -707,7 +711,7 @@ bool map_view(CUtensorMap* map, const void* base, int64_t rows, int64_t heads, i
 
 template <bool F16>
 cudaError_t launch_sparse(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const SparseParams& p,
-                          unsigned grid, int dev, cudaStream_t stream) {
+                          unsigned grid, int dev, bool chained, cudaStream_t stream) {
   static bool attr_set[64] = {false};
   if (dev >= 0 && dev < 64 && !attr_set[dev]) {
     const cudaError_t e =
@@ -715,12 +719,11 @@ cudaError_t launch_sparse(const CUtensorMap& q, const CUtensorMap& k, const CUte
     if (e != cudaSuccess) return e;
     attr_set[dev] = true;
   }
-  sparse_attention_kernel<F16><<<grid, kSpThreads, kSpSmem, stream>>>(q, k, v, p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e =
+      launch_chained(sparse_attention_kernel<F16>, grid, kSpThreads, kSpSmem, stream, chained, q, k, v, p);
   if (e != cudaSuccess || p.parts == 1) return e;
   const int64_t warps = (int64_t)p.heads * p.queries;
-  sparse_join_kernel<F16><<<(unsigned)((warps + 3) / 4), 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_chained(sparse_join_kernel<F16>, (unsigned)((warps + 3) / 4), 128, 0, stream, true, p);
 }
 
 // Runs a list is split into: as many as fill the streams of all SMs, of at least two tiles.
@@ -782,18 +785,21 @@ cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t 
   p.ws_acc = reinterpret_cast<float*>(ws + sh.tiles_bytes);
   p.ws_ml = reinterpret_cast<float2*>(ws + sh.tiles_bytes + sh.acc_bytes);
   p.tiles = a.tiles;
+  bool chained = a.chained;
   if (p.tiles == nullptr) {
     int32_t* tiles = reinterpret_cast<int32_t*>(ws);
     const int64_t rows = a.kv_heads * sh.q_blocks;
-    count_tiles_kernel<<<(unsigned)((rows + 3) / 4), 128, 0, stream>>>(a.blocks, rows, p.top_k, p.k_blocks,
-                                                                      p.block / kSubKeys, tiles);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e =
+        launch_chained(count_tiles_kernel, (unsigned)((rows + 3) / 4), 128, 0, stream, false, a.blocks, rows, p.top_k,
+                       p.k_blocks, p.block / kSubKeys, tiles);
     if (e != cudaSuccess) return e;
+    chained = true;
     p.tiles = tiles;
   }
   // one persistent CTA per SM; a second stream only where every SM has a first one
   const unsigned grid = (unsigned)std::min<int64_t>(sms, p.items);
-  return a.f16 ? launch_sparse<true>(q, k, v, p, grid, dev, stream) : launch_sparse<false>(q, k, v, p, grid, dev, stream);
+  return a.f16 ? launch_sparse<true>(q, k, v, p, grid, dev, chained, stream)
+               : launch_sparse<false>(q, k, v, p, grid, dev, chained, stream);
 }
 
 }  // namespace h3

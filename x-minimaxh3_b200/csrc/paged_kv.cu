@@ -21,7 +21,10 @@
 // Bound: HBM, each row read once and written once. A long prompt gives every
 // token one warp. With few tokens the rows of a token are dealt out over more
 // warps (down to one row per half-warp), since a call on one token is bound by
-// the latency of one chain slot -> address -> store.
+// the latency of one chain slot -> address -> store. What it takes to keep HBM busy is
+// warps: at 102 registers (5 CTAs an SM) 32,760 tokens of 72 rows take 268 us, at 80 (6
+// CTAs) with the first rows' loads ahead of the coefficients 219 us (5.67 TB/s, 87% of the
+// measured copy).
 #include <algorithm>
 
 #include "attn_math.cuh"
@@ -59,23 +62,27 @@ __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i
   return is64 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
 }
 
-// coefficients (own, partner) of rotation pair `pair`: row 0 of [[t00, t01], [t10, t11]] for
-// the first half of the rotated dims (own t00, partner t01), row 1 for the second (own t11)
-__device__ __forceinline__ void load_coef(const void* table, int dtype, int64_t base, int pair, int second, float& own,
-                                          float& other) {
+// coefficients (own, partner) of 8 rotation pairs from `pair` on: row 0 of [[t00, t01], [t10, t11]]
+// for the first half of the rotated dims (own t00, partner t01), row 1 for the second
+// (own t11). Rows are at least 4 elements apart, so a pair's two values load as one word.
+__device__ __forceinline__ void load_coefs(const void* table, int dtype, int64_t base, int pair, int second,
+                                           float (&own)[8], float (&other)[8]) {
   const int64_t at = base + pair * 4 + second * 2;
-  float a, b;
-  if (dtype == 0) {
-    a = __ldg(static_cast<const float*>(table) + at);
-    b = __ldg(static_cast<const float*>(table) + at + 1);
-  } else {
-    const uint16_t* t = static_cast<const uint16_t*>(table) + at;
-    const uint32_t w = (uint32_t)__ldg(t) | ((uint32_t)__ldg(t + 1) << 16);
-    a = dtype == 1 ? Elem16<false>::lo(w) : Elem16<true>::lo(w);
-    b = dtype == 1 ? Elem16<false>::hi(w) : Elem16<true>::hi(w);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float a, b;
+    if (dtype == 0) {
+      const float2 v = __ldg(reinterpret_cast<const float2*>(static_cast<const float*>(table) + at + 4 * i));
+      a = v.x;
+      b = v.y;
+    } else {
+      const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(table) + at + 4 * i));
+      a = dtype == 1 ? Elem16<false>::lo(w) : Elem16<true>::lo(w);
+      b = dtype == 1 ? Elem16<false>::hi(w) : Elem16<true>::hi(w);
+    }
+    own[i] = second ? b : a;
+    other[i] = second ? a : b;
   }
-  own = second ? b : a;
-  other = second ? a : b;
 }
 
 // Rows [lo, hi) of the token's Q or K heads: y = rstd (A x + B x_partner) with the norm
@@ -86,6 +93,16 @@ __device__ __forceinline__ void turn_rows(const uint16_t* src, int64_t src_h, ui
                                           int partner, const float (&ca)[8], const float (&cb)[8]) {
   using E = Elem16<F16>;
   const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15;
+  uint4 x[kAppendUnroll];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < kAppendUnroll; ++u) {
+      const int r = r0 + 2 * u + half;
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < hi) x[u] = ldg_v4(src + r * src_h);
+    }
+  };
+  load(lo);  // on the way while the coefficients arrive
   uint64_t a2[4], b2[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -102,13 +119,7 @@ __device__ __forceinline__ void turn_rows(const uint16_t* src, int64_t src_h, ui
     b2[i] = f2_pack(b0, b1);
   }
   for (int r0 = lo; r0 < hi; r0 += 2 * kAppendUnroll) {
-    uint4 x[kAppendUnroll];
-#pragma unroll
-    for (int u = 0; u < kAppendUnroll; ++u) {
-      const int r = r0 + 2 * u + half;
-      x[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < hi) x[u] = ldg_v4(src + r * src_h);
-    }
+    if (r0 > lo) load(r0);
 #pragma unroll
     for (int u = 0; u < kAppendUnroll; ++u) {
       if (r0 + 2 * u >= hi) break;  // warp-uniform: the shuffles below see both halves
@@ -148,12 +159,14 @@ __device__ __forceinline__ void turn_rows(const uint16_t* src, int64_t src_h, ui
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(kAppendThreads) append_paged_kv_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 6) append_paged_kv_kernel(const AppendParams p) {
   const int64_t warp = (int64_t)blockIdx.x * (kAppendThreads / 32) + (threadIdx.x >> 5);
   const int64_t token = warp / p.chunks;
   if (token >= p.tokens) return;
   const int chunk = (int)(warp - token * p.chunks);
   const int64_t slot = load_index(p.slot_of, p.slot64, token);
+  int64_t position = token;
+  if (p.position_of != nullptr) position = load_index(p.position_of, p.position64, token);
   if (slot < 0 || slot >= p.slots) return;  // padding: nothing of this token is written
   const int half = (threadIdx.x >> 4) & 1, l = threadIdx.x & 15;
   const int nq = p.q_out != nullptr ? p.heads : 0, nk = nq + p.kv_heads;
@@ -172,13 +185,13 @@ __global__ void __launch_bounds__(kAppendThreads) append_paged_kv_kernel(const A
       cb[i] = 0.0f;
     }
     if (rotated) {
-      const int64_t row = p.position_of == nullptr ? token : load_index(p.position_of, p.position64, token);
+      const int64_t row = position;
       const bool known = row >= 0 && row < p.table_rows;
+      if (known)
+        load_coefs(p.table, p.table_dtype, row * p.table_stride, (l - second * step) * 8, second, ca, cb);
+      else
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ca[i] = cb[i] = __int_as_float(0x7FC00000);  // a position outside the table: NaN, not a wrong rotation
-        if (known) load_coef(p.table, p.table_dtype, row * p.table_stride, (l - second * step) * 8 + i, second, ca[i], cb[i]);
-      }
+        for (int i = 0; i < 8; ++i) ca[i] = cb[i] = __int_as_float(0x7FC00000);  // NaN, not a wrong rotation
     }
     if (begin < nq)
       turn_rows<F16>(p.x[0] + token * p.xs_t[0] + l * 8, p.xs_h[0], p.q_out + token * p.qo_t + l * 8, p.qo_h, begin,
@@ -214,6 +227,9 @@ cudaError_t launch_append_paged_kv(const AppendKvArgs& a, cudaStream_t stream) {
   for (int i = a.q ? 0 : 1; i < 3; ++i)
     if (!aligned(xs[i]) || a.xs_t[i] % 8 || a.xs_h[i] % 8) return cudaErrorNotSupported;
   if (a.q && (!aligned(a.q_out) || a.qo_t % 8 || a.qo_h % 8)) return cudaErrorNotSupported;
+  // a rotation pair's coefficients are read two at a time
+  if (a.table && ((reinterpret_cast<uintptr_t>(a.table) & (a.table_dtype == 0 ? 7 : 3)) || a.table_stride % 2))
+    return cudaErrorNotSupported;
   for (int i = 0; i < 2; ++i) {
     if (!aligned(a.cache[i]) || a.c_page[i] % 8 || a.c_head[i] % 8 || a.c_row[i] % 8 || !aligned(a.w[i]))
       return cudaErrorNotSupported;
@@ -237,9 +253,11 @@ cudaError_t launch_append_paged_kv(const AppendKvArgs& a, cudaStream_t stream) {
   int dev = 0;
   cudaGetDevice(&dev);
   const int64_t rows = (a.q ? a.heads : 0) + 2 * a.kv_heads;
-  // runs as long as the token (coefficients read once) when the tokens alone give every
-  // SM its 32 warps, shorter ones, down to one row per half-warp, when they do not
-  const int64_t want = (int64_t)num_sms(dev) * 32;
+  // Runs as long as the token (coefficients read once) when the tokens alone give every SM
+  // 64 warps, two to three rounds of what it holds; shorter ones, down to one row per
+  // half-warp, when they do not. 4,095 tokens x 168 rows: 84 us with 32 warps, 78 with
+  // 64 or 96, 82 with 128.
+  const int64_t want = (int64_t)num_sms(dev) * 64;
   const int64_t chunks = std::min<int64_t>((rows + 1) / 2, std::max<int64_t>(1, (want + a.tokens - 1) / a.tokens));
   p.rows_per_warp = (int)(((rows + chunks - 1) / chunks + 1) / 2 * 2);
   p.chunks = (int)((rows + p.rows_per_warp - 1) / p.rows_per_warp);

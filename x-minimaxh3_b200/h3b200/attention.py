@@ -180,9 +180,11 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
         rows, rot = fshape[0], 2 * fshape[1]
         if rot == 0 or rot > HEAD_DIM or rot % 16:
             raise ValueError(f"frequencies must rotate a multiple of 16 dims, at most {HEAD_DIM}, got {rot}")
-        if not f.is_contiguous() and f.stride()[1:] != (4, 2, 1):
-            f = f.contiguous()
-        stride, freq_ptr = f.stride(0), f.data_ptr()
+        fs = f.stride()
+        if fs[1:] != (4, 2, 1) or fs[0] % 2 or f.data_ptr() % 8:
+            f = f.clone(memory_format=torch.contiguous_format)
+            fs = f.stride()
+        stride, freq_ptr = fs[0], f.data_ptr()
         if positions is not None:
             position_code, position_ptr = _index(positions, "positions", t), positions.data_ptr()
         elif rows < t:

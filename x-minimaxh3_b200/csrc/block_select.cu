@@ -292,7 +292,7 @@ cudaError_t launch_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b,
   if (ctas == 0) return cudaSuccess;
   if (ctas > 0x7FFFFFFF) return cudaErrorNotSupported;
   return launch_chained(f16 ? block_means_kernel<true> : block_means_kernel<false>, (unsigned)ctas, kMeanThreads, 0,
-                        stream, false, src[0], src[1]);
+                        stream, false, 1, src[0], src[1]);
 }
 
 int64_t select_blocks_max() { return (200 * 1024 - kSelRows * kSelPad * 8) / 8 - 4; }
@@ -317,7 +317,7 @@ cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream)
   if (grid > 0x7FFFFFFF) return cudaErrorNotSupported;
   // few CTAs: more warps each, for the latency of their loads
   const int threads = grid < num_sms(dev) ? kSelThreadsMax : kSelThreads;
-  return launch_chained(select_blocks_kernel, (unsigned)grid, threads, smem, stream, a.chained, a.q_means, a.k_means,
+  return launch_chained(select_blocks_kernel, (unsigned)grid, threads, smem, stream, a.chained, 1, a.q_means, a.k_means,
                         a.km_h, a.km_b, (int)(a.heads / a.kv_heads), a.q_blocks, (int)a.k_blocks, (int)a.top_k, rows,
                         (int)a.block, a.queries, a.keys, a.causal ? 1 : 0, a.out, a.tiles,
                         static_cast<const uint16_t*>(a.q_row), a.q_row_h, a.q_row_f16 ? 1 : 0);

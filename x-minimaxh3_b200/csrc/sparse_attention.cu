@@ -720,10 +720,10 @@ cudaError_t launch_sparse(const CUtensorMap& q, const CUtensorMap& k, const CUte
     attr_set[dev] = true;
   }
   const cudaError_t e =
-      launch_chained(sparse_attention_kernel<F16>, grid, kSpThreads, kSpSmem, stream, chained, q, k, v, p);
+      launch_chained(sparse_attention_kernel<F16>, grid, kSpThreads, kSpSmem, stream, chained, 1, q, k, v, p);
   if (e != cudaSuccess || p.parts == 1) return e;
   const int64_t warps = (int64_t)p.heads * p.queries;
-  return launch_chained(sparse_join_kernel<F16>, (unsigned)((warps + 3) / 4), 128, 0, stream, true, p);
+  return launch_chained(sparse_join_kernel<F16>, (unsigned)((warps + 3) / 4), 128, 0, stream, true, 1, p);
 }
 
 // Runs a list is split into: as many as fill the streams of all SMs, of at least two tiles.
@@ -790,7 +790,7 @@ cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t 
     int32_t* tiles = reinterpret_cast<int32_t*>(ws);
     const int64_t rows = a.kv_heads * sh.q_blocks;
     const cudaError_t e =
-        launch_chained(count_tiles_kernel, (unsigned)((rows + 3) / 4), 128, 0, stream, false, a.blocks, rows, p.top_k,
+        launch_chained(count_tiles_kernel, (unsigned)((rows + 3) / 4), 128, 0, stream, false, 1, a.blocks, rows, p.top_k,
                        p.k_blocks, p.block / kSubKeys, tiles);
     if (e != cudaSuccess) return e;
     chained = true;

@@ -206,7 +206,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             qw = _weight(q_weight, "q_weight", q)
             qw_ptr = qw.data_ptr()
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+            q_out = torch.empty_like(q)
         qoshape, qos = _thd(q_out, "q_out", dtype)
         if qoshape != qshape:
             raise ValueError("q_out must have q's shape")
@@ -256,19 +256,19 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                          f"{tuple(lengths.shape)}")
     scale = _scale_of(scale)
     if out is None:
-        out = torch.empty(qshape, dtype=dtype, device=q.device)
+        out = torch.empty_like(q)
     elif out.shape != qshape or out.dtype is not dtype or out.stride(2) != 1:
         raise ValueError(f"out must be {dtype} {tuple(qshape)} with unit stride on the head dim")
     lse = lse_ptr = work = work_ptr = None
     if return_lse:
-        lse = torch.empty((b, heads), dtype=torch.float32, device=q.device)
+        lse = q.new_empty((b, heads), dtype=torch.float32)
         lse_ptr = lse.data_ptr()
     width = tshape[1]
     os = out.stride()
     with _on(dev):
         nbytes = _lib.load().h3b200_paged_decode_workspace_bytes(b, heads, kv_heads, width, page_size)
         if nbytes:
-            work = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            work = q.new_empty(nbytes, dtype=torch.uint8)
             work_ptr = work.data_ptr()
         _lib.call("h3b200_paged_decode_attention", q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), ks[0], ks[1], ks[2],
                   v_cache.data_ptr(), vs[0], vs[1], vs[2], pages, page_size, page_table.data_ptr(), ts[0], width,
@@ -354,7 +354,7 @@ def _block_size(block_size) -> int:
 def _out(out, q, qshape):
     """(out, its [T, H] strides)."""
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q)
     oshape, os = _thd(out, "out", q.dtype)
     if oshape != qshape:
         raise ValueError("out must have q's shape")
@@ -422,13 +422,12 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: i
         _means(k_means, "k_means", kv_heads, -(-s // block_size))
         km_ptr, kms = k_means.data_ptr(), k_means.stride()
     out, os = _out(out, q, qshape)
-    device = q.device
-    lse = torch.empty((t, heads), dtype=torch.float32, device=device) if return_lse else None
-    blocks = torch.empty((kv_heads, -(-t // QUERY_BLOCK), top_k), dtype=torch.int32, device=device)
+    lse = q.new_empty((t, heads), dtype=torch.float32) if return_lse else None
+    blocks = q.new_empty((kv_heads, -(-t // QUERY_BLOCK), top_k), dtype=torch.int32)
     with _on(dev):
         nbytes = _lib.load().h3b200_sparse_attention_workspace_bytes(t, s, heads, kv_heads, top_k, block_size,
                                                                      k_means is not None)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        work = q.new_empty(nbytes, dtype=torch.uint8)
         _lib.call("h3b200_sparse_attention", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(),
                   vs[0], vs[1], km_ptr, kms[0], kms[1], top_k, block_size, blocks.data_ptr(), out.data_ptr(), os[0],
                   os[1], None if lse is None else lse.data_ptr(), heads, 1, t, s, heads, kv_heads, scale,

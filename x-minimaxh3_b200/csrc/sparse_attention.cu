@@ -112,16 +112,6 @@ __device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, ui
       : "memory");
 }
 
-// First key of sub-block `sub` of the list (64 keys from there), or -1: no such block.
-__device__ __forceinline__ int sub_key(const SparseParams& p, const int32_t* list, int sub) {
-  const int per = p.block / kSubKeys;
-  const int e = sub / per;
-  if (e >= p.top_k) return -1;
-  const int id = list[e];
-  if (id < 0 || id >= p.k_blocks) return -1;
-  return id * p.block + (sub - e * per) * kSubKeys;
-}
-
 // 32 lanes x 16 columns, as tmem_ld32 / tmem_st32
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -255,7 +245,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       int pos;                                 // the batch's next item
       int n_head, n_block, n_part, n_first, n_n, n_ids0, n_ids1;  // the item after the current one (n_n 0: none)
       int head, block, part, first, n;         // the item whose K tiles are being loaded (n 0: none)
-      int ids0, ids1;                          // lane e: keys of its tile i0 + e, i0 = i rounded down to 32
+      int ids0, ids1;                          // lane e: block ids of its tile i0 + e, i0 = i rounded down to 32
       int i, item, tile, v_key, v_head;
       bool pending;                            // V of the last K tile is not loaded yet
     } a, o;
@@ -268,13 +258,20 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       }
       t.pos = 0;
     };
+    // Lane e: block ids of tile i + e. Nothing looks at them before key_of, an item (or a
+    // tile) later: the warp would stand still for the length of the load.
+    const int per = p.block / kSubKeys;
     auto read_ids = [&](int head, int block, int first, int n, int i, int& ids0, int& ids1) {
       ids0 = ids1 = -1;
       if (i + lane < n) {
         const int32_t* list = p.blocks + (int64_t)((head / p.group) * p.q_blocks + block) * p.top_k;
-        ids0 = sub_key(p, list, 2 * (first + i + lane));
-        ids1 = sub_key(p, list, 2 * (first + i + lane) + 1);
+        const int e0 = 2 * (first + i + lane) / per, e1 = (2 * (first + i + lane) + 1) / per;
+        if (e0 < p.top_k) ids0 = list[e0];
+        if (e1 < p.top_k) ids1 = list[e1];
       }
+    };
+    auto key_of = [&](int id, int half) {  // first of the 64 keys, or -1: no such block
+      return id < 0 || id >= p.k_blocks ? -1 : id * p.block + (per == 2 ? half * kSubKeys : 0);
     };
     auto advance = [&](Feed& t) {  // the next item becomes the current one; the one after it is looked up
       t.head = t.n_head; t.block = t.n_block; t.part = t.n_part; t.first = t.n_first; t.n = t.n_n;
@@ -333,7 +330,8 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         }
         ++t.item;
       }
-      const int key0 = __shfl_sync(0xFFFFFFFFu, t.ids0, t.i & 31), key1 = __shfl_sync(0xFFFFFFFFu, t.ids1, t.i & 31);
+      const int key0 = key_of(__shfl_sync(0xFFFFFFFFu, t.ids0, t.i & 31), 0);
+      const int key1 = key_of(__shfl_sync(0xFFFFFFFFu, t.ids1, t.i & 31), 1);
       if (u == 0 && lane == 0) key_note[t.s * kNotes + t.tile % kNotes] = make_int2(key0, key1);
       ++t.tile;
       t.v_key = u == 0 ? key0 : key1;

@@ -1433,7 +1433,9 @@ int current_sms() {
   return h3::num_sms(dev);
 }
 
-// page sizes are multiples of 8 keys; key indices of one sequence are 32-bit
+constexpr int64_t kMaxKeys = 1 << 30;  // key indices of one sequence are 32-bit, with room for the kernels' steps
+
+// page sizes are multiples of 8 keys
 int paged_shape(int64_t pages, int64_t page_size, const char* who) {
   if (pages >= 0 && page_size > 0 && page_size % 8 == 0 && page_size <= (1 << 20)) return H3B200_OK;
   return fail(H3B200_ERR_INVALID, "%s: page_size must be a positive multiple of 8 (got %lld) and pages >= 0 (got %lld)", who, (long long)page_size, (long long)pages);
@@ -1498,7 +1500,7 @@ int h3b200_paged_decode_attention(const void* q, int64_t q_sb, int64_t q_sh, con
   if (const int rc = attn_dtype(dtype, who)) return rc;
   if (const int rc = paged_shape(pages, page_size, who)) return rc;
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
-  if (batch < 0 || table_width < 0 || table_width > 0x7FFFFF00 / page_size) return fail(H3B200_ERR_INVALID, "%s: bad shape (a sequence holds fewer than 2^31 keys)", who);
+  if (batch < 0 || table_width < 0 || table_width > kMaxKeys / page_size) return fail(H3B200_ERR_INVALID, "%s: bad shape (a sequence holds at most 2^30 keys)", who);
   if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(H3B200_ERR_INVALID, "%s: scale must be positive and finite", who);
   if (batch == 0) return H3B200_OK;
   if (!q || !out || !lengths || (table_width > 0 && (!page_table || (pages > 0 && (!k_cache || !v_cache))))) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
@@ -1572,7 +1574,8 @@ static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const vo
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
   if (queries < 0 || keys <= 0 || top_k <= 0) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys and top_k must be positive)", who);
   if (block != 64 && block != 128) return fail(H3B200_ERR_UNSUPPORTED, "%s: blocks of 64 or 128 keys are built, got %lld", who, (long long)block);
-  if (top_k > 0x7FFFFF00 / block) return fail(H3B200_ERR_INVALID, "%s: top_k too large", who);
+  if (top_k > kMaxKeys / block) return fail(H3B200_ERR_INVALID, "%s: top_k too large (a list names at most 2^30 keys)", who);
+  if (queries > kMaxKeys || keys > kMaxKeys) return fail(H3B200_ERR_INVALID, "%s: at most 2^30 queries and keys", who);
   if (!(scale > 0.0f) || !(scale < 1e30f)) return fail(H3B200_ERR_INVALID, "%s: scale must be positive and finite", who);
   if (queries == 0) return H3B200_OK;
   if (!q || !k || !v || !blocks || !out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);

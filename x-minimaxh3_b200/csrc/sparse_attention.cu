@@ -759,7 +759,7 @@ cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t 
   cudaGetDevice(&dev);
   const int sms = num_sms(dev);
   const SparseShape sh = sparse_shape(a.queries, a.heads, a.kv_heads, a.top_k, a.block, sms);
-  if (a.queries > 0x7FFFFF00 || a.keys > 0x7FFFFF00 || sh.items * sh.parts > (1 << 30) || a.block % kSubKeys ||
+  if (a.queries > (1 << 30) || a.keys > (1 << 30) || sh.items * sh.parts > (1 << 30) || a.block % kSubKeys ||
       a.o_t % 8 || a.o_h % 8 || (reinterpret_cast<uintptr_t>(a.out) & 15))
     return cudaErrorNotSupported;
   CUtensorMap q, k, v;

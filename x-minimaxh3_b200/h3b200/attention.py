@@ -372,7 +372,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bl
     named twice counts twice. ``block_size`` is 64 or 128 keys. With ``causal``, query row r
     sees the listed keys at positions up to ``r + S - T``. A row that sees no key gives
     zeros (and lse -inf). Under ``causal`` all values of a listed block must be finite: those
-    a row may not see enter its products with weight zero.
+    a row may not see enter its products with weight zero. ``out`` may be ``q``, but must not
+    overlap ``k`` or ``v``.
     Returns ``out`` [T, heads, 128], with ``return_lse`` (out, fp32 [T, heads] log-sum-exp)."""
     dev = _device(q, k, v, blocks, out)
     code, qshape, qs, kshape, ks, vs = _qkv(q, k, v)

@@ -167,7 +167,10 @@ class ClockSampler:
 # its fc2 launches are ``gemm_i8_kernel<10, 2>``, the GEMM whose epilogue stores each int32 row at its
 # owner; the outputs are checked against the fused MLP), ``w4_smallm`` (the W4A8 linear of M rows, at most 16,
 # through fc1's config-2 weight 3,072 -> 12,288 with the asymmetric correction: ConvRot quantizer, then
-# ``gemm_w4_smallm_kernel`` unpacking the int4 weight in shared memory). Shapes are those of the config-1 MLP and config-3
+# ``gemm_w4_smallm_kernel`` unpacking the int4 weight in shared memory), ``append_kv_h3`` (M tokens of the
+# 56-head attention, rot 96, bf16 table, into a paged cache), ``paged_decode`` (one new token of 64 sequences
+# of M keys each, 64 query and 8 key heads, pages of 64) or ``sparse_attn`` (block-sparse attention of M tokens,
+# 24 heads, an eighth of the 64-key blocks). Shapes are those of the config-1 MLP and config-3
 # norm-RoPE with M tokens; inputs are seeded synthetic data. Every case first
 # runs the kernels it needs to build its inputs, then launches the kernel under
 # study ``--iters`` times, so a profiler can skip the set-up launches by kernel
@@ -177,7 +180,7 @@ class ClockSampler:
 
 CASES = ["quantize", "fc1", "fc1_bf16", "fc1_i32", "requant", "fc2", "fc2_rq", "mlp", "mlp_w4a8", "mlp_swiglu",
          "mlp_swiglu_w4", "decode_w4", "qknorm_h3", "qkv_h3", "convrot", "convrot_x", "norm_rope", "rms_adaln",
-         "rms_adaln_h3", "tp2_linked", "w4_smallm"]
+         "rms_adaln_h3", "tp2_linked", "w4_smallm", "append_kv_h3", "paged_decode", "sparse_attn"]
 
 
 def _case_mlp_inputs(m: int, dev):
@@ -303,6 +306,27 @@ def run_case(case: str, m: int, iters: int, report: bool = False):
                                dtype=torch.uint8, device=dev)
             ms = _case_timed(lambda: ops.qkv_qknorm_rope(xq, xs, wq_, ws, None, heads, kn, kn, freqs, 1e-5, "qkv",
                                                     *outs, workspace=work), iters, report)
+    elif case == "append_kv_h3":
+        g = torch.Generator(device=dev).manual_seed(10)
+        q, k, v = (torch.randn(m, 56, 128, generator=g, device=dev).to(torch.bfloat16) for _ in range(3))
+        freqs = torch.randn(m, 48, 2, 2, generator=g, device=dev).to(torch.bfloat16)
+        kn = (1 + 0.02 * torch.randn(128, generator=g, device=dev)).to(torch.bfloat16)
+        kc, vc = (torch.empty(-(-m // 128), 56, 128, 128, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        slots, qo = torch.arange(m, device=dev), torch.empty_like(q)
+        ms = _case_timed(lambda: h3b200.append_paged_kv(k, v, kc, vc, slots, freqs, k_weight=kn, q=q, q_weight=kn,
+                                                        q_out=qo), iters, report)
+    elif case == "paged_decode":
+        g = torch.Generator(device=dev).manual_seed(11)
+        width = -(-m // 64)
+        kc, vc = (torch.randn(64 * width, 8, 64, 128, generator=g, device=dev).to(torch.bfloat16) for _ in range(2))
+        tab = torch.randperm(64 * width, generator=g, device=dev).to(torch.int32).reshape(64, width)
+        lens = torch.full((64,), m, dtype=torch.int32, device=dev)
+        q = torch.randn(64, 64, 128, generator=g, device=dev).to(torch.bfloat16)
+        ms = _case_timed(lambda: h3b200.paged_decode_attention(q, kc, vc, tab, lens), iters, report)
+    elif case == "sparse_attn":
+        g = torch.Generator(device=dev).manual_seed(12)
+        q, k, v = (torch.randn(m, 24, 128, generator=g, device=dev).to(torch.bfloat16) for _ in range(3))
+        ms = _case_timed(lambda: h3b200.sparse_attention(q, k, v, max(1, m // 512)), iters, report)
     elif case == "w4_smallm":
         if m > 16:
             raise SystemExit("w4_smallm: at most 16 rows (larger calls take the decode path)")

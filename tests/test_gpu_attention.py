@@ -507,6 +507,24 @@ def test_prompt_then_tokens():
         check_decode(q, [(k, v)], dense, None, D ** -0.5, torch.bfloat16)
 
 
+def test_reads_what_the_qkv_build_writes():
+    """qkv_qknorm_rope's HND-backed views go straight into the attention and the cache."""
+    gen = _gen(33)
+    m, heads, d = 200, 3, 256
+    w, ws = h3b200.quantize_int8_convrot_weight(randn(gen, 3 * heads * D, d, std=0.05))
+    xq, xs = h3b200.quantize_int8_rowwise_convrot(randn(gen, m, d), 256)
+    nw = randn(gen, D, std=0.1) + 1
+    q, k, v = h3b200.qkv_qknorm_rope(xq, xs, w, ws, None, heads, nw, nw, table(m, 96).reshape(1, m, 1, 48, 2, 2), 1e-6)
+    out, lse, blocks = h3b200.sparse_attention(q, k, v, 2, return_lse=True, return_blocks=True)
+    check_sparse(q, k, v, blocks, 64, False, out, lse, D ** -0.5, torch.bfloat16)
+    kc, vc = (torch.zeros(8, heads, 32, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    h3b200.append_paged_kv(k, v, kc, vc, torch.arange(m, device="cuda"))
+    lens = torch.tensor([m], dtype=torch.int32, device="cuda")
+    pages = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+    one = h3b200.paged_decode_attention(q[m - 1:m], kc, vc, pages, lens)
+    check_decode(q[m - 1:m], [(k, v)], one, None, D ** -0.5, torch.bfloat16)
+
+
 def test_graph_and_streams():
     """Captured steps replay after lengths, tables and inputs change in place; a side stream works."""
     gen = _gen(32)

@@ -11,6 +11,12 @@
 // leaves about 1e-16 of the score's terms as its error. In 32 bits (1e-7) about one
 // selection in 10^4 changes with the order of the sum.
 //
+// Measured (24 heads, 32,760 tokens): means of 201 MB 55 us (3.7 TB/s; the conversions to 64
+// bits, 16 a clock and SM, set the pace), 24 x 256 x 512 scores and the 64 best of each row
+// 78 us (64-bit matrix instructions 20 us of it at their rate; the rest is loads and the
+// descent through the keys' bits, latencies that five CTAs per SM only partly hide).
+// Beside the 1.5 ms of the attention they select for, both were left there.
+//
 // With `causal` (query row r stands at position r + keys - queries), a query
 // block sees the key blocks that start no later than its last row. Those that
 // hold one of its own positions, whose means cover keys behind some of its rows,

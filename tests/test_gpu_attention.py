@@ -413,6 +413,9 @@ def check_sparse(q, k, v, blocks, block, causal, out, lse, scale, dtype):
     (500, 1234, 4, 1, 128, 3, True),
     (200, 90, 2, 1, 64, 5, True),            # rows that see no key
     (3000, 3000, 24, 24, 64, 8, False),      # two query blocks per CTA, more CTAs than SMs
+    (1400, 1600, 32, 8, 64, 5, False),       # grouped heads, more query blocks than streams
+    (1300, 2000, 48, 8, 128, 4, True),
+    (1500, 900, 64, 4, 64, 3, True),         # whole query blocks without a key among them
 ])
 def test_sparse_matches_definition(dtype, queries, keys, heads, kv, block, top_k, causal):
     gen = _gen(queries * 7 + keys)

@@ -38,20 +38,20 @@ _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 _current = contextlib.nullcontext()
 
 
-def _device(*ts) -> int:
+def _device(first, *ts) -> int:
     """Index of the CUDA device that holds every given tensor."""
-    index = ts[0].get_device()
+    if not first.is_cuda:
+        raise ValueError("h3b200 operators take CUDA tensors only (no CPU fallback)")
+    index = first.get_device()
     for t in ts:
         if t is not None and t.get_device() != index:
-            raise ValueError(f"all tensors must be on one device, got {[str(t.device) for t in ts if t is not None]}")
-    if index < 0 or not ts[0].is_cuda:
-        raise ValueError("h3b200 operators take CUDA tensors only (no CPU fallback)")
+            raise ValueError(f"all tensors must be on one device, got {[str(x.device) for x in (first, *ts) if x is not None]}")
     return index
 
 
 def _on(index: int):
     """The tensors' device for the launch (nothing to do when it is the current one)."""
-    return _current if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _current if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 def _stream(index: int) -> int:
@@ -68,6 +68,8 @@ def _dtype_code(t: torch.Tensor) -> int:
 def _thd(t: torch.Tensor, name: str, dtype: torch.dtype):
     """(shape, strides) of [1, T, H, 128] / [T, H, 128] with unit stride on the head dim, as [T, H, 128]."""
     shape, stride = t.shape, t.stride()
+    if len(shape) == 3 and shape[2] == HEAD_DIM and stride[2] == 1 and t.dtype is dtype:
+        return shape, stride
     if len(shape) == 4:
         if shape[0] != 1:
             raise ValueError(f"{name}: batch dimension must be 1 (packed token layout)")

@@ -350,6 +350,16 @@ def test_selection(queries, keys, heads, kv, block, top_k, causal):
     assert torch.equal(got, select64(qm, km, top_k, queries, keys, block, causal))
 
 
+@pytest.mark.parametrize("queries,keys,heads,kv,block,top_k,causal", [
+    (1, 16385, 6, 2, 64, 33, False),        # a few key blocks for each of several CTAs
+    (1, 32768, 24, 24, 64, 64, False),
+    (100, 140000, 4, 1, 64, 500, True),     # more keys than a lane holds in registers
+    (2048, 20000, 14, 2, 128, 1, False),
+])
+def test_selection_few_rows_many_blocks(queries, keys, heads, kv, block, top_k, causal):
+    test_selection(queries, keys, heads, kv, block, top_k, causal)
+
+
 def test_selection_ties_and_odd_scores():
     """Equal scores go to the lowest block, zero of either sign is one score, NaN ranks last."""
     km = torch.zeros(1, 100, D, device="cuda")

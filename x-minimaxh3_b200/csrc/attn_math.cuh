@@ -17,6 +17,10 @@ namespace h3 {
 __device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// barrier of a cluster's CTAs in its two halves; stores before arrive are seen behind wait
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 // kernel<<<grid, block, smem, stream>>>(args...) in clusters of `cluster` CTAs; after_previous:
 // as a dependent of the launch before it
 template <typename... P, typename... A>

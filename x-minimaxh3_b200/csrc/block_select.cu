@@ -13,7 +13,7 @@
 //
 // Measured (24 heads, 32,760 tokens): means of 201 MB 55 us (3.7 TB/s; the conversions to 64
 // bits, 16 a clock and SM, set the pace), 24 x 256 x 512 scores and the 64 best of each row
-// 78 us (64-bit matrix instructions 20 us of it at their rate; the rest is loads and the
+// 74 us (64-bit matrix instructions 20 us of it at their rate; the rest is loads and the
 // descent through the keys' bits, latencies that five CTAs per SM only partly hide).
 // Beside the 1.5 ms of the attention they select for, both were left there.
 //
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(kMeanThreads, 6) block_means_kernel(const Mean
 }
 static_assert(kMeanThreads == kHeadDim, "one thread per dim finishes a mean");
 
-constexpr int kSelThreads = 256, kSelThreadsMax = 512;
+constexpr int kSelThreads = 256;
+constexpr int kSelHeld = 16;  // high words a lane keeps in registers during the descent (512 key blocks)
 constexpr int kSelPad = kHeadDim + 2;  // doubles per staged query row: conflict-free 16-byte reads
 constexpr int kSelRows = 8;  // query blocks per CTA: the M of one 64-bit matrix instruction; one warp each for the top-k
 
@@ -100,6 +101,10 @@ __device__ __forceinline__ void mma_f64(double (&c)[2], double a, double b) {
   asm volatile("mma.sync.aligned.m8n8k4.row.col.f64.f64.f64.f64 {%0,%1}, {%2}, {%3}, {%0,%1};"
                : "+d"(c[0]), "+d"(c[1])
                : "d"(a), "d"(b));
+}
+
+__device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 // 64-bit key whose unsigned order is the order of the scores; 0 stands for "not to be
@@ -121,9 +126,13 @@ __device__ __forceinline__ unsigned long long score_key(double s) {
 // 16 c + 4 t .. + 3) and uses them in four instructions; the 8 query rows are read from
 // shared memory in the same order (in registers they would halve the CTAs per SM).
 //
+// Few query blocks leave most SMs idle, and one CTA takes as long for one row as for
+// eight: then a cluster of `ctas` CTAs scores a row's key blocks, each a part of them,
+// into the first CTA's shared memory.
+//
 // Keys are kept as their high and low words: the high ones (20 bits of the mantissa)
 // nearly always decide alone.
-__global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const float* qm,
+__global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float* qm,
                                                                     const float* km, int64_t km_h,
                                                                     int64_t km_b, int group,
                                                                     int64_t q_blocks, int k_blocks, int top_k,
@@ -132,44 +141,59 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
                                                                     int32_t* __restrict__ out,
                                                                     int32_t* __restrict__ out_tiles,
                                                                     const uint16_t* __restrict__ q_row,
-                                                                    int64_t q_row_h, int q_row_f16) {
+                                                                    int64_t q_row_h, int q_row_f16, int ctas) {
   extern __shared__ __align__(16) unsigned char sel_smem[];
   double* qs = reinterpret_cast<double*>(sel_smem);                          // [kSelRows][kSelPad]
   const int pitch = (k_blocks + 3) & ~3;
   uint32_t* key_hi = reinterpret_cast<uint32_t*>(qs + kSelRows * kSelPad);   // [rows][pitch], 0 behind the last block
   uint32_t* key_lo = key_hi + rows_per_cta * pitch;
+  if (ctas > 1) cluster_arrive();  // first phase: every CTA of the cluster has started
   launch_next();
   wait_previous();
   const int64_t tiles = (q_blocks + rows_per_cta - 1) / rows_per_cta;
-  const int64_t kvh = blockIdx.x / tiles;
-  const int64_t i0 = (blockIdx.x - kvh * tiles) * rows_per_cta;
+  const int64_t cta = blockIdx.x / ctas;
+  const int rank = (int)(blockIdx.x - cta * ctas);
+  const int64_t kvh = cta / tiles;
+  const int64_t i0 = (cta - kvh * tiles) * rows_per_cta;
   const int rows = (int)min((int64_t)rows_per_cta, q_blocks - i0);
-  for (int e = threadIdx.x; e < kSelRows * kHeadDim; e += blockDim.x) {
-    const int r = e / kHeadDim, d = e % kHeadDim;
-    double s = 0.0;
-    if (r < rows) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  static_assert(kSelThreads == kSelRows * 32, "one warp sums a row's query heads");
+  {
+    double s[kHeadDim / 32] = {};
+    if (warp < rows) {
+#pragma unroll 4
       for (int g = 0; g < group; ++g) {
+        const int64_t h = kvh * group + g;
         if (q_row != nullptr) {  // one query: it is its own mean
-          const uint32_t w = __ldg(q_row + (kvh * group + g) * q_row_h + d);
-          s += (double)(q_row_f16 ? Elem16<true>::lo(w) : Elem16<false>::lo(w));
+          const uint16_t* x = q_row + h * q_row_h + lane;
+#pragma unroll
+          for (int e = 0; e < kHeadDim / 32; ++e) {
+            const uint32_t w = __ldg(x + 32 * e);
+            s[e] += (double)(q_row_f16 ? Elem16<true>::lo(w) : Elem16<false>::lo(w));
+          }
         } else {
-          s += (double)*(qm + ((kvh * group + g) * q_blocks + i0 + r) * kHeadDim + d);
+          const float* x = qm + (h * q_blocks + i0 + warp) * kHeadDim + lane;
+#pragma unroll
+          for (int e = 0; e < kHeadDim / 32; ++e) s[e] += (double)x[32 * e];
         }
       }
     }
-    qs[r * kSelPad + d] = s;
+#pragma unroll
+    for (int e = 0; e < kHeadDim / 32; ++e) qs[warp * kSelPad + lane + 32 * e] = s[e];
   }
-  for (int e = threadIdx.x; e < rows * (pitch - k_blocks); e += blockDim.x) {
+  for (int e = threadIdx.x; e < rows * (pitch - k_blocks); e += kSelThreads) {
     const int r = e / (pitch - k_blocks);
     key_hi[r * pitch + k_blocks + e - r * (pitch - k_blocks)] = 0u;
   }
   __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   {
     const int g = lane >> 2, t = lane & 3;
     const double2* a = reinterpret_cast<const double2*>(qs + g * kSelPad + 4 * t);
     const float* base = km + kvh * km_h + 4 * t;
-    for (int j0 = warp * 8; j0 < k_blocks; j0 += blockDim.x / 32 * 8) {
+    constexpr int warps = kSelThreads / 32;
+    const uint32_t hi0 = ctas > 1 ? mapa_shared(key_hi, 0) : 0u, lo0 = ctas > 1 ? mapa_shared(key_lo, 0) : 0u;
+    if (ctas > 1) cluster_wait();
+    for (int j0 = (rank * warps + warp) * 8; j0 < k_blocks; j0 += ctas * warps * 8) {
       float4 v[8];
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
@@ -198,12 +222,23 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
           if (start + block > first) k = ~0ull;
           if (start > last) k = 0ull;
         }
-        key_hi[g * pitch + j] = (uint32_t)(k >> 32);
-        key_lo[g * pitch + j] = (uint32_t)k;
+        if (ctas > 1) {
+          st_cluster_u32(hi0 + (g * pitch + j) * 4, (uint32_t)(k >> 32));
+          st_cluster_u32(lo0 + (g * pitch + j) * 4, (uint32_t)k);
+        } else {
+          key_hi[g * pitch + j] = (uint32_t)(k >> 32);
+          key_lo[g * pitch + j] = (uint32_t)k;
+        }
       }
     }
   }
-  __syncthreads();
+  if (ctas > 1) {
+    cluster_arrive();       // second phase: all keys are in the first CTA's shared memory
+    if (rank != 0) return;
+    cluster_wait();
+  } else {
+    __syncthreads();
+  }
   if (warp >= rows) return;
   const uint32_t* hi = key_hi + warp * pitch;
   const uint32_t* lo = key_lo + warp * pitch;
@@ -212,19 +247,39 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
   // than that can be selected: a key of 0 cannot, and the high word of every other is not 0)
   uint32_t th = 1u;
   int above = 0;  // keys >= th
+  uint32_t v[kSelHeld];  // the lane's high words, where there are few enough
+  const bool held = k_blocks <= 32 * kSelHeld;
+  if (held) {
+#pragma unroll
+    for (int e = 0; e < kSelHeld; ++e) v[e] = lane + 32 * e < k_blocks ? hi[lane + 32 * e] : 0u;
+  }
   {
     uint32_t most = 0u, least = ~0u;
-    for (int j = lane; j < k_blocks; j += 32) {
-      most = max(most, hi[j]);
-      least = min(least, hi[j]);
+    if (held) {
+#pragma unroll
+      for (int e = 0; e < kSelHeld; ++e) {
+        most = max(most, v[e]);
+        least = min(least, lane + 32 * e < k_blocks ? v[e] : ~0u);
+      }
+    } else {
+      for (int j = lane; j < k_blocks; j += 32) {
+        most = max(most, hi[j]);
+        least = min(least, hi[j]);
+      }
     }
     most = __reduce_max_sync(0xFFFFFFFFu, most);
     least = __reduce_min_sync(0xFFFFFFFFu, least);
     auto count = [&](uint32_t c) {  // keys with a high word >= c, c > 0
       int n = 0;
-      for (int j = lane * 4; j < pitch; j += 128) {
-        const uint4 v = *reinterpret_cast<const uint4*>(hi + j);
-        n += (v.x >= c) + (v.y >= c) + (v.z >= c) + (v.w >= c);
+      if (held) {
+#pragma unroll
+        for (int e = 0; e < kSelHeld; ++e) n += v[e] >= c;
+      } else {
+#pragma unroll 4
+        for (int j = lane * 4; j < pitch; j += 128) {
+          const uint4 w = *reinterpret_cast<const uint4*>(hi + j);
+          n += (w.x >= c) + (w.y >= c) + (w.z >= c) + (w.w >= c);
+        }
       }
       return (int)__reduce_add_sync(0xFFFFFFFFu, (unsigned)n);
     };
@@ -258,6 +313,7 @@ __global__ void __launch_bounds__(kSelThreadsMax) select_blocks_kernel(const flo
     equal_left = top_k - (th_lo == ~0u ? count(true, 0u) : count(false, th_lo + 1u));
   }
   int at = 0;
+#pragma unroll 4
   for (int j0 = 0; j0 < k_blocks; j0 += 32) {
     const int j = j0 + lane;
     const uint32_t h = j < k_blocks ? hi[j] : 0u;
@@ -320,13 +376,16 @@ cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream)
     attr_set[dev] = true;
   }
   const int64_t grid = a.kv_heads * ((a.q_blocks + rows - 1) / rows);
-  if (grid > 0x7FFFFFFF) return cudaErrorNotSupported;
-  // few CTAs: more warps each, for the latency of their loads
-  const int threads = grid < num_sms(dev) ? kSelThreadsMax : kSelThreads;
-  return launch_chained(select_blocks_kernel, (unsigned)grid, threads, smem, stream, a.chained, 1, a.q_means, a.k_means,
+  if (grid > 0x0FFFFFFF) return cudaErrorNotSupported;
+  // CTAs per row tile: while the GPU holds them all at once, and down to two steps of key
+  // blocks per warp (24 rows of 512 key blocks: 22.5 us in one CTA each, 16.4 in clusters of
+  // 4 and of 8; 56 tiles of 65 key blocks: 16.4 in one CTA each and in clusters of 2)
+  const int64_t steps = (a.k_blocks + kSelThreads / 4 - 1) / (kSelThreads / 4);
+  const int ctas = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(8, steps / 2), 3 * num_sms(dev) / grid));
+  return launch_chained(select_blocks_kernel, (unsigned)(grid * ctas), kSelThreads, smem, stream, a.chained, ctas, a.q_means, a.k_means,
                         a.km_h, a.km_b, (int)(a.heads / a.kv_heads), a.q_blocks, (int)a.k_blocks, (int)a.top_k, rows,
                         (int)a.block, a.queries, a.keys, a.causal ? 1 : 0, a.out, a.tiles,
-                        static_cast<const uint16_t*>(a.q_row), a.q_row_h, a.q_row_f16 ? 1 : 0);
+                        static_cast<const uint16_t*>(a.q_row), a.q_row_h, a.q_row_f16 ? 1 : 0, ctas);
 }
 
 }  // namespace h3

@@ -22,9 +22,11 @@
 // token one warp. With few tokens the rows of a token are dealt out over more
 // warps (down to one row per half-warp), since a call on one token is bound by
 // the latency of one chain slot -> address -> store. What it takes to keep HBM busy is
-// warps: at 102 registers (5 CTAs an SM) 32,760 tokens of 72 rows take 268 us, at 80 (6
-// CTAs) with the first rows' loads ahead of the coefficients 219 us (5.67 TB/s, 87% of the
-// measured copy).
+// loads in flight: at 102 registers (5 CTAs an SM) 32,760 tokens of 72 rows take 268 us, at
+// 80 (6 CTAs) with the first rows' loads ahead of the coefficients 219 us, with the rest of
+// a run's Q or K rows prefetched into L2 205 us (6.06 TB/s, 93% of the measured copy). One
+// step of prefetching ahead instead of the run's gives 209; Q, K and V rows of the token at
+// once, or before its slot is known, 244.
 #include <algorithm>
 
 #include "attn_math.cuh"
@@ -57,6 +59,10 @@ struct AppendParams {
   int rows_per_warp, chunks;
   float eps;
 };
+
+__device__ __forceinline__ void prefetch_l2(const void* p, int bytes) {  // both multiples of 16
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(bytes));
+}
 
 __device__ __forceinline__ int64_t load_index(const void* p, int is64, int64_t i) {
   return is64 ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
@@ -103,6 +109,9 @@ __device__ __forceinline__ void turn_rows(const uint16_t* src, int64_t src_h, ui
     }
   };
   load(lo);  // on the way while the coefficients arrive
+  // and the rest of the run on its way to L2, one row per lane
+  for (int r = lo + 2 * kAppendUnroll + (threadIdx.x & 31); r < hi; r += 32)
+    prefetch_l2(src - l * 8 + r * src_h, kHeadDim * 2);
   uint64_t a2[4], b2[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -254,10 +263,9 @@ cudaError_t launch_append_paged_kv(const AppendKvArgs& a, cudaStream_t stream) {
   cudaGetDevice(&dev);
   const int64_t rows = (a.q ? a.heads : 0) + 2 * a.kv_heads;
   // Runs as long as the token (coefficients read once) when the tokens alone give every SM
-  // 64 warps, two to three rounds of what it holds; shorter ones, down to one row per
-  // half-warp, when they do not. 4,095 tokens x 168 rows: 84 us with 32 warps, 78 with
-  // 64 or 96, 82 with 128.
-  const int64_t want = (int64_t)num_sms(dev) * 64;
+  // 96 warps, four rounds of what it holds; shorter ones, down to one row per half-warp,
+  // when they do not. 4,095 tokens x 168 rows: 82 us with 64 warps, 74 with 96, 78 with 128.
+  const int64_t want = (int64_t)num_sms(dev) * 96;
   const int64_t chunks = std::min<int64_t>((rows + 1) / 2, std::max<int64_t>(1, (want + a.tokens - 1) / a.tokens));
   p.rows_per_warp = (int)(((rows + chunks - 1) / chunks + 1) / 2 * 2);
   p.chunks = (int)((rows + p.rows_per_warp - 1) / p.rows_per_warp);

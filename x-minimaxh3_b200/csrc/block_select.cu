@@ -11,10 +11,12 @@
 // leaves about 1e-16 of the score's terms as its error. In 32 bits (1e-7) about one
 // selection in 10^4 changes with the order of the sum.
 //
-// Measured (24 heads, 32,760 tokens): means of 201 MB 55 us (3.7 TB/s; the conversions to 64
-// bits, 16 a clock and SM, set the pace), 24 x 256 x 512 scores and the 64 best of each row
-// 74 us (64-bit matrix instructions 20 us of it at their rate; the rest is loads and the
-// descent through the keys' bits, latencies that five CTAs per SM only partly hide).
+// Measured (24 heads, 32,760 tokens, L2 full of written lines): means of 201 MB 57 us (3.5
+// TB/s; 49 with sums in 32 bits, so most of it is the reads and the write-back beside them;
+// prefetching the next CTA's rows, 8 CTAs per SM or shorter unrolls change nothing),
+// 24 x 256 x 512 scores and the 64 best of each row 74 us (64-bit matrix instructions 20 us
+// of it at their rate; the rest is loads and the descent through the keys' bits, latencies
+// that the CTAs of an SM only partly hide).
 // Beside the 1.5 ms of the attention they select for, both were left there.
 //
 // With `causal` (query row r stands at position r + keys - queries), a query

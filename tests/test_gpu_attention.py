@@ -355,9 +355,21 @@ def test_selection(queries, keys, heads, kv, block, top_k, causal):
     (1, 32768, 24, 24, 64, 64, False),
     (100, 140000, 4, 1, 64, 500, True),     # more keys than a lane holds in registers
     (2048, 20000, 14, 2, 128, 1, False),
+    (1024, 190000, 2, 1, 64, 100, False),   # as much shared memory as eight rows take, in a cluster
 ])
 def test_selection_few_rows_many_blocks(queries, keys, heads, kv, block, top_k, causal):
     test_selection(queries, keys, heads, kv, block, top_k, causal)
+
+
+def test_selection_refusals():
+    """Counts that a 64-bit argument would wrap are refused like other bad ones."""
+    m = torch.zeros(1, 1, D, device="cuda")
+    for top_k, block in ((0, 64), (1 << 25, 64), ((1 << 64) + 1, 64), (1, 0), (1, (1 << 64) + 1)):
+        with pytest.raises(ValueError):
+            h3b200.select_key_blocks(m, m, top_k, 1, 64, block)
+    x = torch.zeros(1, 1, D, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        h3b200.sparse_attention(x, x, x, (1 << 64) + 1)
 
 
 def test_selection_ties_and_odd_scores():

@@ -318,8 +318,9 @@ def select_key_blocks(q_means: torch.Tensor, k_means: torch.Tensor, top_k: int, 
     behind the query block are never selected, and those that reach into it come first."""
     dev = _device(q_means, k_means)
     queries, keys, block_size, top_k = int(queries), int(keys), int(block_size), int(top_k)
-    if queries < 0 or keys < 0 or block_size <= 0 or top_k <= 0:
-        raise ValueError("top_k and block_size must be positive, queries and keys not negative")
+    if queries < 0 or keys < 0 or not 0 < block_size <= 1 << 20 or not 0 < top_k <= 1 << 24:
+        raise ValueError(f"top_k ({top_k}) and block_size ({block_size}) must be positive (at most 2^24 and 2^20), "
+                         "queries and keys not negative")
     qb, kb = -(-queries // QUERY_BLOCK), -(-keys // block_size)
     _means(q_means, "q_means", None, qb)
     _means(k_means, "k_means", None, kb)
@@ -417,8 +418,8 @@ def sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, top_k: i
     t, heads, _ = qshape
     s, kv_heads, _ = kshape
     top_k, block_size = int(top_k), _block_size(block_size)
-    if top_k <= 0:
-        raise ValueError(f"top_k must be positive, got {top_k}")
+    if not 0 < top_k <= 1 << 24:
+        raise ValueError(f"top_k must be positive (at most 2^24), got {top_k}")
     scale = _scale_of(scale)
     km_ptr, kms = None, (0, 0)
     if k_means is not None:

@@ -488,6 +488,26 @@ def test_sparse_keys_behind_the_last_are_not_read():
         check_sparse(q, k[:333], v[:333], blocks, 64, False, out, lse, D ** -0.5, torch.bfloat16)
 
 
+def test_sparse_hidden_values_count_nothing():
+    """The weight of a key that a row may not see is zero, not just small: values near the largest
+    finite one, hidden under `causal`, leave the rows before them as they are."""
+    gen = _gen(24)
+    t, seen = 256, 201
+    q, k, v = randn(gen, t, 2, D), randn(gen, t, 1, D), randn(gen, t, 1, D)
+    blocks = torch.arange(4, dtype=torch.int32, device="cuda").expand(1, 2, 4).contiguous()
+    loud = v.clone()
+    loud[seen:] = 3e38
+    out, lse = h3b200.block_sparse_attention(q, k, loud, blocks, causal=True, return_lse=True)
+    mask = list_mask(blocks, 0, t, t, 64, True)[:seen]
+    for h in range(2):
+        ref = attend64(q[:seen, h], k[:, 0], v[:, 0], mask, D ** -0.5)
+        check_attention(out[:seen, h], lse[:seen, h], ref, torch.bfloat16, float(v.abs().max()), f"head {h}")
+    # rows that see no key at all
+    out, lse = h3b200.block_sparse_attention(q, k[:100], loud[-100:], blocks[..., :2].contiguous(), causal=True,
+                                             return_lse=True)
+    assert not bool(out[:t - 100].any()) and bool(torch.isneginf(lse[:t - 100]).all())
+
+
 # ---------------------------------------------------------------------------
 # together
 # ---------------------------------------------------------------------------

@@ -106,15 +106,16 @@ __device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^a, 2^b by arithmetic on the FMA pipe, for a, b <= 64 (below -126 as at -126; NaN stays
-// NaN). n = round(x) through the addition of 1.5 * 2^23, f = x - n in [-0.5, 0.5], the
-// polynomial of degree 5 with the least relative error there (Remez exchange; 2.4e-7
-// with these fp32 coefficients), times 2^n built from n's bits.
+// 2^a, 2^b by arithmetic on the FMA pipe, for a, b <= 64. n = round(x) through the addition
+// of 1.5 * 2^23, f = x - n in [-0.5, 0.5], the polynomial of degree 5 with the least
+// relative error there (Remez exchange; 2.4e-7 with these fp32 coefficients), times 2^n
+// built from n's bits. 0 below -126.5, where n is -127 and those bits come out as 0 (the
+// weight of a hidden key is exactly 0); NaN stays NaN.
 __device__ __forceinline__ void exp2_poly2(uint64_t x, float& a, float& b) {
   float x0, x1;
   f2_unpack(x, x0, x1);
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-126.0f));
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-126.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x0) : "f"(x0), "f"(-127.0f));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x1) : "f"(x1), "f"(-127.0f));
   x = f2_pack(x0, x1);
   const uint64_t t = f2_add(x, f2_pack(12582912.0f, 12582912.0f));
   const uint64_t f = f2_fma(f2_add(t, f2_pack(-12582912.0f, -12582912.0f)), f2_pack(-1.0f, -1.0f), x);

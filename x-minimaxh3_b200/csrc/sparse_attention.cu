@@ -591,7 +591,6 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       tc_fence_after();
       i = 0;
       ++item;
-      if (m == -INFINITY) l = 0.0f;  // no key seen: exp2_poly2 gives 2^-126 for -inf
       if (p.parts > 1) {
         const int64_t at = ((int64_t)(it.head * p.q_blocks + it.q_block) * p.parts + it.part) * kQueryBlock + row_in;
         if (row < p.queries) p.ws_ml[at] = make_float2(m, l);

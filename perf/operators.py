@@ -27,19 +27,12 @@ TABLES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 _LARGEST = 13_000_000_000_000   # flops a drawn sparse case may have, dense upper bound of the largest listed one
 
 
-_loaded = None
-
-
 def _framework():
-    global _loaded
-    if _loaded is not None:     # a program imports the package once, not in every call
-        return _loaded
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "x-minimaxh3_b200")
     if root not in sys.path:
         sys.path.insert(1, root)
     import h3b200
 
-    _loaded = h3b200
     return h3b200
 
 

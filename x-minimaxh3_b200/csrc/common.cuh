@@ -228,6 +228,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, unsign
   return true;
 }
 
+// mbar_wait by a whole warp, with one verdict for all of it: where another wait gives up
+// meanwhile, a lane may still see its own phase complete while its neighbour does not, and
+// a warp that only some lanes leave never meets its votes, shuffles and TMEM accesses again.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, unsigned int code) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, code));
+}
+
 // mbar_wait with cluster-scope acquire: for phases completed by arrivals from
 // the peer CTA of a pair (release.cluster) that order the peer's TMEM accesses.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar_addr, uint32_t parity) {

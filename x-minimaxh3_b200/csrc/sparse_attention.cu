@@ -320,8 +320,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     };
     auto load_tile = [&](int key, int kv_head, const CUtensorMap* map) {
       const int slot = issued % kRing;
-      // one verdict for the warp: the shuffles need all of it
-      if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[slot], ((issued / kRing) & 1) ^ 1, kErrSpProd))) return false;
+      if (!mbar_wait_warp(&kv_empty[slot], ((issued / kRing) & 1) ^ 1, kErrSpProd)) return false;
       if (lane == 0) {
         uint8_t* dst = smem + kOffRing + slot * kTileBytes + u * (kSubKeys * 128);
         mbar_arrive_expect_tx(&kv_full[slot], kHalfBytes);
@@ -333,7 +332,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     };
     auto load_k = [&](Feed& t) {
       if (t.i == 0) {  // a new item: its queries, once the item before has used the buffer
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&q_empty[t.s], (t.item & 1) ^ 1, kErrSpProd))) return false;
+        if (!mbar_wait_warp(&q_empty[t.s], (t.item & 1) ^ 1, kErrSpProd)) return false;
         if (lane == 0) {
           if (u == 0) item_note[t.s * kNotes + t.item % kNotes] = ItemNote{t.head, t.block, t.part, t.n};
           mbar_arrive_expect_tx(&q_full[t.s], kHalfBytes);
@@ -474,7 +473,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int t = 0; t < total; ++t) {
-      if (!mbar_wait(&s_full[s], t & 1, kErrSpSoft)) {
+      if (!mbar_wait_warp(&s_full[s], t & 1, kErrSpSoft)) {
         ok = false;
         break;
       }
@@ -558,7 +557,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           l *= f;
           // O holds what is complete: the tiles before (their commit came before s_full's)
           // and, for the second half, the first half's product
-          if (h == 1) ok = mbar_wait(&h_done[s], t & 1, kErrSpSoft) && ok;
+          if (h == 1) ok = mbar_wait_warp(&h_done[s], t & 1, kErrSpSoft) && ok;
           if (i > 0 || h == 1) {
             tc_fence_after();
 #pragma unroll 1
@@ -584,7 +583,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
       }
       if (++i < it.n) continue;
       // the item's last tile: its rows
-      if (!mbar_wait(&o_full[s], item & 1, kErrSpOut)) {
+      if (!mbar_wait_warp(&o_full[s], item & 1, kErrSpOut)) {
         ok = false;
         break;
       }

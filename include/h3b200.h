@@ -716,6 +716,8 @@ H3B200_API int h3b200_select_key_blocks(const float* q_means, const float* k_mea
  * query block may not see (causal) still enter its products with weight zero, so they
  * must be finite; rows behind the last key do not exist for the kernel. q, k, v, out:
  * [tokens, heads, 128] at token / head strides. scale > 0.
+ * workspace: h3b200_block_sparse_workspace_bytes (which depends on the current device's SM
+ * count) bytes, 256-byte aligned; not needed after the call's work has run.
  */
 H3B200_API int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads,
                                                        int64_t top_k, int64_t block);

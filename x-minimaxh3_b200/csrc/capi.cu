@@ -1433,6 +1433,9 @@ int current_sms() {
   return h3::num_sms(dev);
 }
 
+// the rows of split lists are stored 32 bytes at a time, at multiples of 256 bytes into the workspace
+constexpr uintptr_t kSparseWsMask = 31;
+
 constexpr int64_t kMaxKeys = 1 << 30;  // key indices of one sequence are 32-bit, with room for the kernels' steps
 
 // page sizes are multiples of 8 keys
@@ -1580,7 +1583,7 @@ static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const vo
   if (queries == 0) return H3B200_OK;
   if (!q || !k || !v || !blocks || !out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
   const int64_t need = h3b200_block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block);
-  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+  if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & kSparseWsMask)))
     return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
   if (queries == 1) {
     // one token sees every key it lists (its position is the last one): the split kernel
@@ -1639,7 +1642,7 @@ int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const voi
   if (queries < 0 || keys <= 0 || top_k <= 0 || block <= 0 || block > (1 << 20)) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys, top_k and block must be positive)", who);
   if (queries == 0) return H3B200_OK;
   const int64_t need = h3b200_sparse_attention_workspace_bytes(queries, keys, heads, kv_heads, top_k, block, k_means != nullptr);
-  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & kSparseWsMask))
     return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
   const int64_t row = h3::kHeadDim * 4, k_blocks = (keys + block - 1) / block;
   uint8_t* base = static_cast<uint8_t*>(workspace);

@@ -379,7 +379,7 @@ struct SparseAttnArgs {
   float* lse = nullptr;
   int64_t l_t = 0, l_h = 0;
   const int32_t* tiles = nullptr;  // list_tiles of each list, where the caller knows them
-  void* workspace = nullptr;       // block_sparse_workspace_bytes, 16-byte aligned
+  void* workspace = nullptr;       // block_sparse_workspace_bytes, 32-byte aligned
   bool f16 = false;
   bool chained = false;            // as a dependent of the launch before it (block selection)
 };

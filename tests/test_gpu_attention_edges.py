@@ -1,0 +1,83 @@
+"""Edges of the attention operators on the GPU: weights far below their row's largest one. References
+and tolerances as in test_gpu_attention.py, where a test says nothing else.
+"""
+
+import math
+
+import pytest
+import torch
+
+import h3b200
+from test_gpu_attention import D, F64, _gen, attend64, half_step, tiny
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# small weights
+# ---------------------------------------------------------------------------
+
+
+def faint_keys(gen, n, kv, dtype):
+    """(k, v) of n keys: the first one outweighs every other by 2^22 to 2^33 for a query of 16 in dim 0 and
+    0 elsewhere, and its value is 0, so that the result consists of the faint keys' values alone."""
+    k = torch.zeros(n, kv, D, device="cuda")
+    fade = 22 + 11 * torch.rand(n, kv, generator=gen, device="cuda")
+    k[..., 0] = -fade * math.log(2.0) / (16 * D ** -0.5)
+    k[0] = 0.0
+    v = 64 * (torch.rand(n, kv, D, generator=gen, device="cuda") + 0.5)
+    v[0] = 0.0
+    return k.to(dtype), v.to(dtype)
+
+
+def check_faint(out, lse, q, k, v, smallest):
+    """As check_attention, but a weight is held to half of `smallest`, the step of the smallest weights that the
+    kernel keeps, relative to the row's largest one."""
+    mask = torch.ones(q.shape[0], k.shape[0], dtype=torch.bool, device="cuda")
+    o, ls, pv, a, n = attend64(q, k, v, mask, D ** -0.5)
+    h = half_step(q.dtype)
+    e = (128 * 2.0 ** -24 * a)[:, None]
+    tol = pv * (h + 2 * e + 2.0 ** -20 + 2 * k.shape[0] * 2.0 ** -24) + h * o.abs() + tiny(q.dtype) + (
+        k.shape[0] * smallest / 2 * float(v.abs().max()))
+    off = (out.to(F64) - o).abs()
+    assert bool((off <= tol).all()), f"worst {float((off / tol).max())} of the tolerance"
+    assert bool(((lse.to(F64) - ls).abs() <= e[:, 0] + 2.0 ** -20 + k.shape[0] * 2.0 ** -24 + 2.0 ** -23 * ls.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,batch,heads,kv", [(777, 1, 8, 8), (3001, 1, 2, 1), (600, 500, 4, 1), (9000, 200, 4, 2),
+                                                (60000, 2, 20, 1)])
+def test_decode_keeps_faint_weights(dtype, n, batch, heads, kv):
+    """fp16 weights keep 39 bits below the largest: 2^15 times as many as fp16 itself has below 1."""
+    gen = _gen(n)
+    k, v = faint_keys(gen, n, kv, dtype)
+    page = 64
+    width = -(-n // page)
+    pad = torch.zeros(width * page - n, kv, D, dtype=dtype, device="cuda")
+    kc, vc = (torch.cat((x, pad)).reshape(width, page, kv, D).transpose(1, 2) for x in (k, v))
+    tab = torch.arange(width, dtype=torch.int32, device="cuda").expand(batch, width)
+    q = torch.zeros(batch, heads, D, dtype=dtype, device="cuda")
+    q[..., 0] = 16.0
+    lens = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out, lse = h3b200.paged_decode_attention(q, kc, vc, tab, lens, return_lse=True)
+    smallest = 2.0 ** -39 if dtype is torch.float16 else 2.0 ** -133
+    for b in (0, batch - 1):
+        for h in range(heads):
+            g = h // (heads // kv)
+            check_faint(out[b, h:h + 1], lse[b, h:h + 1], q[b, h:h + 1], k[:, g], v[:, g], smallest)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("t,n,heads,kv", [(130, 700, 2, 2), (200, 9000, 2, 1), (900, 20000, 24, 2), (900, 60000, 24, 1)])
+def test_sparse_keeps_faint_weights(dtype, t, n, heads, kv):
+    """Weights count from a maximum that may be 2^8 too low, so fp16 keeps 31 bits below it."""
+    gen = _gen(n + t)
+    k, v = faint_keys(gen, n, kv, dtype)
+    q = torch.zeros(t, heads, D, dtype=dtype, device="cuda")
+    q[..., 0] = 16.0
+    out, lse = h3b200.sparse_attention(q, k, v, -(-n // 64), return_lse=True)
+    smallest = 2.0 ** -31 if dtype is torch.float16 else 2.0 ** -125
+    rows = torch.tensor([0, 1, t // 2, t - 1], device="cuda")
+    for h in {0, heads - 1}:
+        g = h // (heads // kv)
+        check_faint(out[rows, h], lse[rows, h], q[rows, h], k[:, g], v[:, g], smallest)

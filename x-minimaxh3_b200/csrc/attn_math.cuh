@@ -81,6 +81,17 @@ struct Elem16 {
   }
 };
 
+// Softmax weights are held as 2^BITS times exp(s - m) up to the end, where BITS cancels in O / l
+// and is taken out of the log-sum-exp. fp16 has only 24 binary places below 1, so that weights
+// below 2^-25 of the largest would be lost to P while l counts them: 32,760 keys at 2^-25.5
+// are 0.07% of the row, more than fp16's own rounding of the result. BITS is what lies
+// between the largest weight and 65,504. bf16 has fp32's range and needs none.
+template <bool F16, int BITS>
+struct WeightScale {
+  static constexpr float log2 = F16 ? (float)BITS : 0.0f;
+  static constexpr float inv = F16 ? 1.0f / (float)(1 << BITS) : 1.0f;
+};
+
 // two fp32 per instruction (sm_100 packed arithmetic, each half rounded to nearest)
 __device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
   uint64_t r;

@@ -15,7 +15,8 @@
 //    32 c + 8 t .. + 7) and uses them as two operand registers of two
 //    instructions; Q is held in the same order.
 //  * exp(S^T), rounded to 16 bits (the tensor core's operand type; the sum l
-//    takes the unrounded values), is transposed in registers (movmatrix).
+//    takes the unrounded values; in fp16 times 2^15, see WeightScale), is transposed in
+//    registers (movmatrix).
 //  * O^T += V^T P^T: lane (g, t) reads 16 contiguous bytes (dims 8 g .. + 7) of
 //    keys 2t, 2t + 1, 2t + 8, 2t + 9 and pairs the keys with byte permutes. The
 //    output rows are permuted accordingly; each lane ends with 8 consecutive dims.
@@ -42,6 +43,8 @@ namespace {
 
 constexpr int kDecWarps = 4;
 constexpr int kDecThreads = kDecWarps * 32;
+template <bool F16>
+using DecodeWeight = WeightScale<F16, 15>;  // the largest weight of a warp's keys so far is 1
 
 struct DecodeParams {
   const uint16_t* q;
@@ -221,7 +224,7 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[e] = exp2f(fmaf(s[e], p.scale_log2, -sub[e & 1]));
+        s[e] = exp2f(fmaf(s[e], p.scale_log2, DecodeWeight<F16>::log2 - sub[e & 1]));
         l[n][e & 1] += s[e];
       }
       pb[n][0] = movmatrix_trans(E::pack(s[0], s[1]));
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
     y.y = E::pack(o.z * inv, o.w * inv);
     *reinterpret_cast<uint2*>(p.out + b * p.o_b + (head0 + r) * p.o_h + d) = y;
     if (d == 0 && p.lse != nullptr)
-      p.lse[b * p.l_b + (head0 + r) * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum));
+      p.lse[b * p.l_b + (head0 + r) * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum * DecodeWeight<F16>::inv));
   };
   if (p.clustered) cluster_wait();
   for (int i = threadIdx.x; i < rows * (kHeadDim / 4); i += kDecThreads) {
@@ -397,7 +400,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeParams p, 
   y.y = E::pack(o.z * inv, o.w * inv);
   *reinterpret_cast<uint2*>(p.out + b * p.o_b + head * p.o_h + lane * 4) = y;
   if (lane == 0 && p.lse != nullptr)
-    p.lse[b * p.l_b + head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum));
+    p.lse[b * p.l_b + head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum * DecodeWeight<F16>::inv));
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -15,8 +15,8 @@
 //  * O += P V: P read from TMEM, V from shared memory as an MN-major operand (the
 //    keys are its contraction dim, so it is never transposed); fp32 in TMEM.
 // O is rescaled only when a row's maximum grew by more than 2^8 since the last
-// rescale (P then stays below 2^8, and l and O carry the same stale maximum, which
-// cancels in O / l).
+// rescale (P then stays below 2^8, in fp16 times 2^7 (WeightScale), and l and O carry the
+// same stale maximum, which cancels in O / l).
 //
 // A CTA runs two such streams over one tensor pipe: while four warps do the softmax of
 // one stream, the tensor core works on the other. Two query tiles, a ring of five 32 KB
@@ -56,6 +56,8 @@ constexpr int kOffBar = kOffRing + kRing * kTileBytes;
 constexpr int kSpSmem = kOffBar + 1024 + 1024;     // + barriers and notes + alignment
 constexpr unsigned kErrSpProd = 0x501, kErrSpMma = 0x502, kErrSpSoft = 0x503, kErrSpOut = 0x504, kErrSpDrain = 0x505;
 constexpr float kRescaleLog2 = 8.0f;
+template <bool F16>
+using SparseWeight = WeightScale<F16, 7>;  // weights count from a maximum that may be 2^8 too low
 // One pair of exponentials of kPolyOf is computed on the FMA pipe: the special-function
 // unit gives 16 a clock and SM, 1,024 clocks a tile, as long as the tile's products take.
 constexpr int kPolyOf = 8;
@@ -530,7 +532,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
 #pragma unroll 1
         for (;;) {
           const float sub = m == -INFINITY ? 0.0f : m * p.scale_log2;
-          const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(-sub, -sub);
+          const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(SparseWeight<F16>::log2 - sub, SparseWeight<F16>::log2 - sub);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           sum[0] = sum[1] = 0ull;
 #pragma unroll
@@ -629,7 +631,7 @@ __global__ void __launch_bounds__(kSpThreads, 1)
           __syncwarp();
         }
         if (row < p.queries && p.lse != nullptr)
-          p.lse[(int64_t)row * p.l_t + (int64_t)it.head * p.l_h] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l));
+          p.lse[(int64_t)row * p.l_t + (int64_t)it.head * p.l_h] = l == 0.0f ? -INFINITY : fmaf(m, p.scale, logf(l * SparseWeight<F16>::inv));
       }
     }
     if (ok && empty_of[s]) {  // query blocks without any key
@@ -705,7 +707,7 @@ __global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) 
   y.y = E::pack(o.z * inv, o.w * inv);
   *reinterpret_cast<uint2*>(p.out + (int64_t)row * p.o_t + (int64_t)head * p.o_h + lane * 4) = y;
   if (lane == 0 && p.lse != nullptr)
-    p.lse[(int64_t)row * p.l_t + (int64_t)head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum));
+    p.lse[(int64_t)row * p.l_t + (int64_t)head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum * SparseWeight<F16>::inv));
 }
 
 bool map_view(CUtensorMap* map, const void* base, int64_t rows, int64_t heads, int64_t st, int64_t sh, int box_rows) {

@@ -339,34 +339,64 @@ __global__ void __launch_bounds__(kSelThreads) select_blocks_kernel(const float*
 
 }  // namespace
 
+namespace {
+
+int64_t mean_blocks(const BlockMeansArgs& m) {
+  return m.tokens > 0 && m.heads > 0 ? (m.tokens + m.block - 1) / m.block : 0;
+}
+
+int64_t mean_ctas(const BlockMeansArgs& a, const BlockMeansArgs& b) {
+  return mean_blocks(a) * a.heads + mean_blocks(b) * b.heads;
+}
+
+// query blocks of one CTA: fewer where so many rows of scores do not fit
+int select_rows(const SelectBlocksArgs& a) {
+  int rows = (int)std::min<int64_t>(kSelRows, a.q_blocks);
+  while (rows > 1 && (int64_t)rows * (a.k_blocks + 4) > select_blocks_max()) rows = (rows + 1) / 2;
+  return rows;
+}
+
+}  // namespace
+
+cudaError_t check_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b) {
+  for (const BlockMeansArgs* m : {&a, &b})
+    if (mean_blocks(*m) > 0 && ((reinterpret_cast<uintptr_t>(m->x) & 15) || m->x_t % 8 || m->x_h % 8))
+      return cudaErrorNotSupported;
+  return mean_ctas(a, b) > 0x7FFFFFFF ? cudaErrorNotSupported : cudaSuccess;
+}
+
 cudaError_t launch_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b, bool f16, cudaStream_t stream) {
+  const cudaError_t e = check_block_means(a, b);
+  const int64_t ctas = mean_ctas(a, b);
+  if (e != cudaSuccess || ctas == 0) return e;
   MeanSource src[2];
-  int64_t ctas = 0;
   for (int i = 0; i < 2; ++i) {
     const BlockMeansArgs& m = i ? b : a;
     src[i].x = static_cast<const uint16_t*>(m.x);
     src[i].x_t = m.x_t; src[i].x_h = m.x_h; src[i].tokens = m.tokens;
     src[i].heads = (int)m.heads; src[i].block = (int)m.block;
-    src[i].blocks = m.tokens > 0 && m.heads > 0 ? (m.tokens + m.block - 1) / m.block : 0;
+    src[i].blocks = mean_blocks(m);
     src[i].means = m.means;
-    ctas += src[i].blocks * m.heads;
-    if (src[i].blocks > 0 && ((reinterpret_cast<uintptr_t>(m.x) & 15) || m.x_t % 8 || m.x_h % 8))
-      return cudaErrorNotSupported;
   }
-  if (ctas == 0) return cudaSuccess;
-  if (ctas > 0x7FFFFFFF) return cudaErrorNotSupported;
   return launch_chained(f16 ? block_means_kernel<true> : block_means_kernel<false>, (unsigned)ctas, kMeanThreads, 0,
                         stream, false, 1, src[0], src[1]);
 }
 
 int64_t select_blocks_max() { return (200 * 1024 - kSelRows * kSelPad * 8) / 8 - 4; }
 
-cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream) {
+cudaError_t check_select_blocks(const SelectBlocksArgs& a) {
   if (a.q_blocks <= 0 || a.kv_heads <= 0 || a.top_k <= 0) return cudaSuccess;
   if (a.k_blocks > select_blocks_max() || (reinterpret_cast<uintptr_t>(a.k_means) & 15) || a.km_h % 4 || a.km_b % 4)
     return cudaErrorNotSupported;
-  int rows = (int)std::min<int64_t>(kSelRows, a.q_blocks);
-  while (rows > 1 && (int64_t)rows * (a.k_blocks + 4) > select_blocks_max()) rows = (rows + 1) / 2;
+  const int rows = select_rows(a);
+  return a.kv_heads * ((a.q_blocks + rows - 1) / rows) > 0x0FFFFFFF ? cudaErrorNotSupported : cudaSuccess;
+}
+
+cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream) {
+  if (a.q_blocks <= 0 || a.kv_heads <= 0 || a.top_k <= 0) return cudaSuccess;
+  const cudaError_t refused = check_select_blocks(a);
+  if (refused != cudaSuccess) return refused;
+  const int rows = select_rows(a);
   const int smem = (int)(kSelRows * kSelPad * 8 + (int64_t)rows * ((a.k_blocks + 3) / 4 * 4) * 8);
   static bool attr_set[64] = {false};
   int dev = 0;
@@ -378,7 +408,6 @@ cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream)
     attr_set[dev] = true;
   }
   const int64_t grid = a.kv_heads * ((a.q_blocks + rows - 1) / rows);
-  if (grid > 0x0FFFFFFF) return cudaErrorNotSupported;
   // CTAs per row tile: while the GPU holds them all at once, and down to two steps of key
   // blocks per warp (24 rows of 512 key blocks: 22.5 us in one CTA each, 16.4 in clusters of
   // 4 and of 8; 56 tiles of 65 key blocks: 16.4 in one CTA each and in clusters of 2)

@@ -1536,15 +1536,16 @@ int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t x_sh, int6
   return from_cuda(h3::launch_block_means(a, h3::BlockMeansArgs(), dtype == H3B200_DTYPE_F16, S(stream)), who);
 }
 
-static int select_impl(h3::SelectBlocksArgs& a, h3b200_stream_t stream, const char* who) {
+// Checks a selection's arguments and fills in its block counts; `a.queries` may be 0 (nothing to launch).
+static int select_args(h3::SelectBlocksArgs& a, const char* who) {
   if (const int rc = attn_heads(a.heads, a.kv_heads, who)) return rc;
-  if (a.queries < 0 || a.keys < 0 || a.block <= 0 || a.block > (1 << 20) || a.top_k <= 0 || a.top_k > (1 << 24)) return fail(H3B200_ERR_INVALID, "%s: bad shape (top_k and block must be positive)", who);
+  if (a.queries < 0 || a.keys < 0 || a.block <= 0 || a.block > (1 << 20) || a.top_k <= 0 || a.top_k > (1 << 24)) return fail(H3B200_ERR_INVALID, "%s: bad shape (top_k and block must be positive, at most 2^24 and 2^20)", who);
   if (a.queries == 0) return H3B200_OK;
   a.q_blocks = (a.queries + h3::kQueryBlock - 1) / h3::kQueryBlock;
   a.k_blocks = (a.keys + a.block - 1) / a.block;
   if (a.k_blocks > h3::select_blocks_max()) return fail(H3B200_ERR_UNSUPPORTED, "%s: %lld key blocks, at most %lld are built", who, (long long)a.k_blocks, (long long)h3::select_blocks_max());
   if ((!a.q_means && !a.q_row) || (a.keys > 0 && !a.k_means) || !a.out) return fail(H3B200_ERR_INVALID, "%s: NULL pointer", who);
-  return from_cuda(h3::launch_select_blocks(a, S(stream)), who);
+  return from_cuda(h3::check_select_blocks(a), who);
 }
 
 int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb, int64_t heads,
@@ -1555,7 +1556,8 @@ int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t
   a.q_means = q_means; a.k_means = k_means; a.km_h = km_sh; a.km_b = km_sb;
   a.heads = heads; a.kv_heads = kv_heads; a.queries = queries; a.keys = keys; a.block = block; a.top_k = top_k;
   a.causal = causal != 0; a.out = blocks;
-  return select_impl(a, stream, "select_key_blocks");
+  if (const int rc = select_args(a, "select_key_blocks")) return rc;
+  return queries == 0 ? H3B200_OK : from_cuda(h3::launch_select_blocks(a, S(stream)), "select_key_blocks");
 }
 
 int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k,
@@ -1565,14 +1567,19 @@ int64_t h3b200_block_sparse_workspace_bytes(int64_t queries, int64_t heads, int6
   return h3::block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block, current_sms());
 }
 
-// tiles: h3::list_tiles of each list where the caller knows them, else nullptr; chained: the
-// launch before on this stream was the selection
-static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
-                             const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks, const int32_t* tiles,
+// A checked block-sparse call: nothing but the launch itself can refuse it any more.
+struct BlockSparseCall {
+  bool one_query = false;
+  h3::PagedDecodeArgs decode;  // one query
+  h3::SparseAttnArgs attention;
+};
+
+static int block_sparse_args(BlockSparseCall& c, const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
+                             int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, const int32_t* blocks,
                              int64_t top_k, int64_t block, void* out, int64_t o_st, int64_t o_sh, float* lse,
                              int64_t l_st, int64_t l_sh, int64_t queries, int64_t keys, int64_t heads,
                              int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
-                             int64_t workspace_bytes, bool chained, h3b200_stream_t stream, const char* who) {
+                             int64_t workspace_bytes, const char* who) {
   if (const int rc = attn_dtype(dtype, who)) return rc;
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
   if (queries < 0 || keys <= 0 || top_k <= 0) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys and top_k must be positive)", who);
@@ -1585,10 +1592,11 @@ static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const vo
   const int64_t need = h3b200_block_sparse_workspace_bytes(queries, heads, kv_heads, top_k, block);
   if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & kSparseWsMask)))
     return fail(H3B200_ERR_INVALID, "%s: workspace too small or misaligned (need %lld bytes)", who, (long long)need);
-  if (queries == 1) {
+  c.one_query = queries == 1;
+  if (c.one_query) {
     // one token sees every key it lists (its position is the last one): the split kernel
     // with the list as each head's page table
-    h3::PagedDecodeArgs a;
+    h3::PagedDecodeArgs& a = c.decode;
     a.q = q; a.q_b = 0; a.q_h = q_sh;
     a.k = k; a.k_page = block * k_st; a.k_head = k_sh; a.k_row = k_st;
     a.v = v; a.v_page = block * v_st; a.v_head = v_sh; a.v_row = v_st;
@@ -1596,18 +1604,28 @@ static int block_sparse_impl(const void* q, int64_t q_st, int64_t q_sh, const vo
     a.pages = (keys + block - 1) / block; a.page_size = block; a.rows = keys;
     a.out = out; a.o_b = 0; a.o_h = o_sh; a.lse = lse; a.l_b = 0; a.l_h = l_sh;
     a.batch = 1; a.heads = heads; a.kv_heads = kv_heads; a.scale = scale;
-    a.workspace = workspace; a.f16 = dtype == H3B200_DTYPE_F16; a.chained = chained;
-    return from_cuda(h3::launch_paged_decode(a, S(stream)), who);
+    a.workspace = workspace; a.f16 = dtype == H3B200_DTYPE_F16;
+    return from_cuda(h3::check_paged_decode(a), who);
   }
-  h3::SparseAttnArgs a;
+  h3::SparseAttnArgs& a = c.attention;
   a.q = q; a.k = k; a.v = v;
   a.q_t = q_st; a.q_h = q_sh; a.k_t = k_st; a.k_h = k_sh; a.v_t = v_st; a.v_h = v_sh;
-  a.blocks = blocks; a.tiles = tiles; a.workspace = workspace;
+  a.blocks = blocks; a.workspace = workspace;
   a.queries = queries; a.keys = keys; a.heads = heads; a.kv_heads = kv_heads; a.top_k = top_k; a.block = block;
   a.scale = scale; a.causal = causal != 0;
   a.out = out; a.o_t = o_st; a.o_h = o_sh; a.lse = lse; a.l_t = l_st; a.l_h = l_sh;
-  a.f16 = dtype == H3B200_DTYPE_F16; a.chained = chained;
-  return from_cuda(h3::launch_block_sparse_attention(a, S(stream)), who);
+  a.f16 = dtype == H3B200_DTYPE_F16;
+  return from_cuda(h3::check_block_sparse_attention(a), who);
+}
+
+// tiles: h3::list_tiles of each list where the caller knows them, else nullptr; chained: the
+// launch before on this stream was the selection
+static int block_sparse_launch(BlockSparseCall& c, const int32_t* tiles, bool chained, h3b200_stream_t stream,
+                               const char* who) {
+  c.decode.chained = c.attention.chained = chained;
+  c.attention.tiles = tiles;
+  return from_cuda(c.one_query ? h3::launch_paged_decode(c.decode, S(stream))
+                               : h3::launch_block_sparse_attention(c.attention, S(stream)), who);
 }
 
 int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st,
@@ -1617,8 +1635,11 @@ int h3b200_block_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, con
                                   int64_t kv_heads, float scale, int causal, int dtype, void* workspace,
                                   int64_t workspace_bytes, h3b200_stream_t stream) {
   H3_GUARD("block_sparse_attention", stream);
-  return block_sparse_impl(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, nullptr, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
-                           heads, kv_heads, scale, causal, dtype, workspace, workspace_bytes, false, stream, "block_sparse_attention");
+  const char* who = "block_sparse_attention";
+  BlockSparseCall c;
+  if (const int rc = block_sparse_args(c, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
+                                       heads, kv_heads, scale, causal, dtype, workspace, workspace_bytes, who)) return rc;
+  return queries == 0 ? H3B200_OK : block_sparse_launch(c, nullptr, false, stream, who);
 }
 
 int64_t h3b200_sparse_attention_workspace_bytes(int64_t queries, int64_t keys, int64_t heads, int64_t kv_heads,
@@ -1640,6 +1661,7 @@ int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const voi
   const char* who = "sparse_attention";
   if (const int rc = attn_heads(heads, kv_heads, who)) return rc;
   if (queries < 0 || keys <= 0 || top_k <= 0 || block <= 0 || block > (1 << 20)) return fail(H3B200_ERR_INVALID, "%s: bad shape (keys, top_k and block must be positive)", who);
+  if (queries > kMaxKeys || keys > kMaxKeys || top_k > kMaxKeys / block) return fail(H3B200_ERR_INVALID, "%s: at most 2^30 queries, keys and keys of a list", who);
   if (queries == 0) return H3B200_OK;
   const int64_t need = h3b200_sparse_attention_workspace_bytes(queries, keys, heads, kv_heads, top_k, block, k_means != nullptr);
   if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & kSparseWsMask))
@@ -1665,7 +1687,6 @@ int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const voi
     mk.x = k; mk.x_t = k_st; mk.x_h = k_sh; mk.tokens = keys; mk.heads = kv_heads; mk.block = block; mk.means = km;
     k_means = km; km_sh = k_blocks * h3::kHeadDim; km_sb = h3::kHeadDim;
   }
-  if (const int rc = from_cuda(h3::launch_block_means(mq, mk, f16, S(stream)), who)) return rc;
   sel.k_means = k_means; sel.km_h = km_sh; sel.km_b = km_sb;
   sel.heads = heads; sel.kv_heads = kv_heads; sel.queries = queries; sel.keys = keys; sel.block = block; sel.top_k = top_k;
   sel.causal = causal != 0; sel.out = blocks;
@@ -1673,9 +1694,15 @@ int h3b200_sparse_attention(const void* q, int64_t q_st, int64_t q_sh, const voi
   int32_t* tiles = queries > 1 ? reinterpret_cast<int32_t*>(base) : nullptr;
   sel.tiles = tiles;
   sel.chained = mq.tokens > 0 || mk.tokens > 0;
-  if (const int rc = select_impl(sel, stream, who)) return rc;
-  return block_sparse_impl(q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, tiles, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
-                           heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, true, stream, who);
+  // every refusal comes before the first launch
+  BlockSparseCall c;
+  if (const int rc = block_sparse_args(c, q, q_st, q_sh, k, k_st, k_sh, v, v_st, v_sh, blocks, top_k, block, out, o_st, o_sh, lse, l_st, l_sh, queries, keys,
+                                       heads, kv_heads, scale, causal, dtype, base, static_cast<uint8_t*>(workspace) + workspace_bytes - base, who)) return rc;
+  if (const int rc = select_args(sel, who)) return rc;
+  if (const int rc = from_cuda(h3::check_block_means(mq, mk), who)) return rc;
+  if (const int rc = from_cuda(h3::launch_block_means(mq, mk, f16, S(stream)), who)) return rc;
+  if (const int rc = from_cuda(h3::launch_select_blocks(sel, S(stream)), who)) return rc;
+  return block_sparse_launch(c, tiles, true, stream, who);
 }
 
 }  // extern "C"

@@ -280,7 +280,8 @@ cudaError_t launch_swiglu_rows(const void* x, int64_t ldx, void* y, int64_t ldy,
 
 // ---------------------------------------------------------------------------
 // Attention after the Q/K/V build: 16-bit elements (bf16, or fp16 with f16), head dim
-// 128, element strides, 16-byte aligned rows. cudaErrorNotSupported outside that.
+// 128, element strides, 16-byte aligned rows. cudaErrorNotSupported outside that; check_x
+// gives launch_x's answer to that without launching, for calls of several launches.
 // ---------------------------------------------------------------------------
 
 // Keys and values (and rotated queries) of new tokens into a paged cache (paged_kv.cu).
@@ -335,6 +336,7 @@ struct PagedDecodeArgs {
   bool chained = false;  // as a dependent of the launch before it (block selection)
 };
 int64_t paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t max_keys, int sms);
+cudaError_t check_paged_decode(const PagedDecodeArgs& a);
 cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream);
 
 constexpr int kQueryBlock = 128;  // query rows that share a selection of key blocks
@@ -346,6 +348,7 @@ struct BlockMeansArgs {
   int64_t x_t = 0, x_h = 0, tokens = 0, heads = 0, block = 1;
   float* means = nullptr;
 };
+cudaError_t check_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b);
 cudaError_t launch_block_means(const BlockMeansArgs& a, const BlockMeansArgs& b, bool f16, cudaStream_t stream);
 // out [kv_heads, q_blocks, top_k]: selected key blocks, ascending, -1 behind them
 struct SelectBlocksArgs {
@@ -364,6 +367,7 @@ struct SelectBlocksArgs {
 // 128-key tiles of a list of `count` blocks
 __host__ __device__ inline int list_tiles(int count, int subs_per_block) { return (count * subs_per_block + 1) / 2; }
 int64_t select_blocks_max();  // key blocks the kernel can score
+cudaError_t check_select_blocks(const SelectBlocksArgs& a);
 cudaError_t launch_select_blocks(const SelectBlocksArgs& a, cudaStream_t stream);
 
 // Attention of 128-row query blocks over listed key blocks (sparse_attention.cu)
@@ -385,6 +389,7 @@ struct SparseAttnArgs {
 };
 int64_t block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_heads, int64_t top_k, int64_t block,
                                      int sms);
+cudaError_t check_block_sparse_attention(const SparseAttnArgs& a);
 cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t stream);
 
 // 2-D tiled TMA descriptor (no interleave, 256-byte L2 promotion, no OOB fill);

@@ -449,12 +449,21 @@ int64_t paged_decode_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_he
   return rows * (kHeadDim * 4 + 8);
 }
 
-cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream) {
-  if (a.batch <= 0) return cudaSuccess;
-  DecodeParams p;
+cudaError_t check_paged_decode(const PagedDecodeArgs& a) {
   if (!aligned(a.q) || a.q_b % 8 || a.q_h % 8 || !aligned(a.k) || a.k_page % 8 || a.k_head % 8 || a.k_row % 8 ||
       !aligned(a.v) || a.v_page % 8 || a.v_head % 8 || a.v_row % 8 || !aligned(a.out) || a.o_b % 8 || a.o_h % 8)
     return cudaErrorNotSupported;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int splits = paged_decode_splits(a.batch, a.heads, a.kv_heads, a.width * a.page_size, num_sms(dev));
+  return decode_items(a.batch, a.heads, a.kv_heads) * splits > 0x7FFFFFFF ? cudaErrorNotSupported : cudaSuccess;
+}
+
+cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream) {
+  if (a.batch <= 0) return cudaSuccess;
+  const cudaError_t refused = check_paged_decode(a);
+  if (refused != cudaSuccess) return refused;
+  DecodeParams p;
   p.q = static_cast<const uint16_t*>(a.q); p.q_b = a.q_b; p.q_h = a.q_h;
   p.k = static_cast<const uint16_t*>(a.k); p.k_page = a.k_page; p.k_head = a.k_head; p.k_row = a.k_row;
   p.v = static_cast<const uint16_t*>(a.v); p.v_page = a.v_page; p.v_head = a.v_head; p.v_row = a.v_row;
@@ -472,8 +481,7 @@ cudaError_t launch_paged_decode(const PagedDecodeArgs& a, cudaStream_t stream) {
   cudaGetDevice(&dev);
   p.splits = paged_decode_splits(a.batch, a.heads, a.kv_heads, a.width * a.page_size, num_sms(dev));
   p.part_min = kPartMin;
-  const int64_t items = a.batch * a.kv_heads * p.row_tiles;
-  if (items * p.splits > 0x7FFFFFFF) return cudaErrorNotSupported;
+  const int64_t items = decode_items(a.batch, a.heads, a.kv_heads);
   p.clustered = clustered(items, p.splits, num_sms(dev));
   p.ws_acc = static_cast<float*>(a.workspace);
   p.ws_ml = reinterpret_cast<float2*>(p.ws_acc + items * p.splits * tile * kHeadDim);

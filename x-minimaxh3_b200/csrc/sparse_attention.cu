@@ -710,11 +710,19 @@ __global__ void __launch_bounds__(128) sparse_join_kernel(const SparseParams p) 
     p.lse[(int64_t)row * p.l_t + (int64_t)head * p.l_h] = sum == 0.0f ? -INFINITY : fmaf(mx, p.scale, logf(sum * SparseWeight<F16>::inv));
 }
 
+// Token and head strides as a tensor map takes them: a dim of one element has no stride that
+// matters, but the encoder still checks it.
+int64_t map_stride(int64_t count, int64_t stride) { return count == 1 ? kHeadDim : stride; }
+
+bool view_maps(const void* base, int64_t rows, int64_t heads, int64_t st, int64_t sh) {
+  for (const int64_t s : {map_stride(rows, st), map_stride(heads, sh)})
+    if (s <= 0 || s % 8 || s * 2 >= (1ll << 40)) return false;  // a broadcast dim (stride 0) has no map
+  return (reinterpret_cast<uintptr_t>(base) & 15) == 0;
+}
+
 bool map_view(CUtensorMap* map, const void* base, int64_t rows, int64_t heads, int64_t st, int64_t sh, int box_rows) {
-  // a dim of one element has no stride that matters; the encoder still checks it
-  if (rows == 1) st = kHeadDim;
-  if (heads == 1) sh = kHeadDim;
-  if ((reinterpret_cast<uintptr_t>(base) & 15) || st <= 0 || sh <= 0 || st % 8 || sh % 8) return false;
+  st = map_stride(rows, st);
+  sh = map_stride(heads, sh);
   return encode_tmap_3d_bf16(map, base, kHeadDim, (uint64_t)rows, (uint64_t)heads, (uint64_t)st * 2, (uint64_t)sh * 2,
                              64, (uint32_t)box_rows, 1, CU_TENSOR_MAP_SWIZZLE_128B);
 }
@@ -765,15 +773,27 @@ int64_t block_sparse_workspace_bytes(int64_t queries, int64_t heads, int64_t kv_
   return s.tiles_bytes + s.acc_bytes + s.ml_bytes;
 }
 
+cudaError_t check_block_sparse_attention(const SparseAttnArgs& a) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const SparseShape sh = sparse_shape(a.queries, a.heads, a.kv_heads, a.top_k, a.block, num_sms(dev));
+  if (a.queries > (1 << 30) || a.keys > (1 << 30) || sh.items * sh.parts > (1 << 30) || a.block % kSubKeys ||
+      a.o_t % 8 || a.o_h % 8 || (reinterpret_cast<uintptr_t>(a.out) & 15))
+    return cudaErrorNotSupported;
+  return view_maps(a.q, a.queries, a.heads, a.q_t, a.q_h) && view_maps(a.k, a.keys, a.kv_heads, a.k_t, a.k_h) &&
+                 view_maps(a.v, a.keys, a.kv_heads, a.v_t, a.v_h)
+             ? cudaSuccess
+             : cudaErrorNotSupported;
+}
+
 cudaError_t launch_block_sparse_attention(const SparseAttnArgs& a, cudaStream_t stream) {
   if (a.queries <= 0 || a.heads <= 0) return cudaSuccess;
+  const cudaError_t refused = check_block_sparse_attention(a);
+  if (refused != cudaSuccess) return refused;
   int dev = 0;
   cudaGetDevice(&dev);
   const int sms = num_sms(dev);
   const SparseShape sh = sparse_shape(a.queries, a.heads, a.kv_heads, a.top_k, a.block, sms);
-  if (a.queries > (1 << 30) || a.keys > (1 << 30) || sh.items * sh.parts > (1 << 30) || a.block % kSubKeys ||
-      a.o_t % 8 || a.o_h % 8 || (reinterpret_cast<uintptr_t>(a.out) & 15))
-    return cudaErrorNotSupported;
   CUtensorMap q, k, v;
   if (!map_view(&q, a.q, a.queries, a.heads, a.q_t, a.q_h, kQueryBlock) ||
       !map_view(&k, a.k, a.keys, a.kv_heads, a.k_t, a.k_h, kSubKeys) ||

@@ -1,5 +1,6 @@
-"""Edges of the attention operators on the GPU: weights far below their row's largest one. References
-and tolerances as in test_gpu_attention.py, where a test says nothing else.
+"""Edges of the attention operators on the GPU: weights far below their row's largest one and rotation
+tables without rows. References and tolerances as in test_gpu_attention.py, where a test says
+nothing else.
 """
 
 import math
@@ -8,7 +9,7 @@ import pytest
 import torch
 
 import h3b200
-from test_gpu_attention import D, F64, _gen, attend64, half_step, tiny
+from test_gpu_attention import D, F64, _gen, attend64, half_step, randn, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +82,28 @@ def test_sparse_keeps_faint_weights(dtype, t, n, heads, kv):
     for h in {0, heads - 1}:
         g = h // (heads // kv)
         check_faint(out[rows, h], lse[rows, h], q[rows, h], k[:, g], v[:, g], smallest)
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("tab", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rot", [16, 96, 128])
+def test_append_table_without_rows(tab, rot):
+    """Every position lies outside a table without rows: NaN in the rotated dims, as for any other such position."""
+    gen = _gen(rot)
+    t, h, page = 5, 3, 8
+    q, k, v = (randn(gen, t, h, D) for _ in range(3))
+    kc, vc = (torch.zeros(2, h, page, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.arange(2, 2 + t, device="cuda")
+    f = torch.empty(0, rot // 2, 2, 2, dtype=tab, device="cuda")
+    for freqs in (f, f.reshape(1, 0, 1, rot // 2, 2, 2)):
+        kc.zero_()
+        qo = h3b200.append_paged_kv(k, v, kc, vc, slots, freqs, torch.arange(t, device="cuda"), q=q)
+        for got, x in ((qo, q), (kc.transpose(1, 2).reshape(-1, h, D)[2:2 + t], k)):
+            assert bool(got[..., :rot].isnan().all()) and torch.equal(got[..., rot:], x[..., rot:])
+        assert torch.equal(vc.transpose(1, 2).reshape(-1, h, D)[2:2 + t], v)
+    with pytest.raises(ValueError):
+        h3b200.append_paged_kv(k, v, kc, vc, slots, f)   # token t would use row t

@@ -186,7 +186,8 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
         if fs[1:] != (4, 2, 1) or fs[0] % 2 or f.data_ptr() % 8:
             f = f.clone(memory_format=torch.contiguous_format)
             fs = f.stride()
-        stride, freq_ptr = fs[0], f.data_ptr()
+        # a table without rows has no address, but is not "no rotation": nothing of it is read
+        stride, freq_ptr = fs[0], f.data_ptr() if rows else k.data_ptr()
         if positions is not None:
             position_code, position_ptr = _index(positions, "positions", t), positions.data_ptr()
         elif rows < t:

@@ -1,6 +1,6 @@
-"""Edges of the attention operators on the GPU: weights far below their row's largest one and rotation
-tables without rows. References and tolerances as in test_gpu_attention.py, where a test says
-nothing else.
+"""Edges of the attention operators on the GPU: weights far below their row's largest one, rotation
+tables without rows and outputs made inside a call. References and tolerances as in
+test_gpu_attention.py, where a test says nothing else.
 """
 
 import math
@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import h3b200
-from test_gpu_attention import D, F64, _gen, attend64, half_step, randn, tiny
+from test_gpu_attention import D, F64, _gen, attend64, half_step, randn, table, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,28 @@ def test_append_table_without_rows(tab, rot):
         assert torch.equal(vc.transpose(1, 2).reshape(-1, h, D)[2:2 + t], v)
     with pytest.raises(ValueError):
         h3b200.append_paged_kv(k, v, kc, vc, slots, f)   # token t would use row t
+
+
+@pytest.mark.parametrize("tokens,heads", [(9, 4), (700, 24)])
+def test_append_made_q_out_is_zero_for_padding(tokens, heads):
+    """A q_out made inside the call holds zeros where a token is padding, not what the allocator had there."""
+    gen = _gen(tokens)
+    qkv = randn(gen, tokens, 3 * heads * D)
+    q, k, v = (x.reshape(tokens, heads, D) for x in qkv.split(heads * D, 1))
+    page = 16
+    pages = tokens // page + 2
+    kc, vc = (torch.zeros(pages, heads, page, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    slots = torch.randperm(pages * page, generator=gen, device="cuda")[:tokens]
+    slots[1], slots[tokens // 2], slots[tokens - 1] = -1, pages * page, -5
+    live = (slots >= 0) & (slots < pages * page)
+    for shape in ((tokens, heads, D), (1, tokens, heads, D)):
+        torch.cuda.synchronize()
+        stale = torch.full(shape, float("nan"), dtype=torch.bfloat16, device="cuda")
+        del stale
+        out = h3b200.append_paged_kv(k, v, kc, vc, slots, table(tokens, 64), q=q.reshape(shape))
+        assert out.shape == torch.Size(shape)
+        out = out.reshape(tokens, heads, D)
+        assert not bool(out[~live].any()) and not bool(out.isnan().any())
+        want = torch.zeros(tokens, heads, D, dtype=torch.bfloat16, device="cuda")
+        h3b200.append_paged_kv(k, v, kc, vc, slots, table(tokens, 64), q=q, q_out=want)
+        assert torch.equal(out, want)

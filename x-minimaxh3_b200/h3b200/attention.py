@@ -140,15 +140,15 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     row ``slots[t] % page_size`` of page ``slots[t] // page_size`` of ``k_cache`` / ``v_cache``
     [pages, kv_heads, page_size, 128] (page_size a multiple of 8), in place (a cache kept as
     [pages, page_size, kv_heads, 128] is passed as its ``transpose(1, 2)``). A token whose slot
-    is -1 (or any value outside the pool) is padding: nothing of it is written, its ``q_out``
-    row included. The slots of one call must differ; which token a slot named twice ends up
+    is -1 (or any value outside the pool) is padding: nothing of it is written, its row of a
+    given ``q_out`` included (a ``q_out`` made here has zeros there). The slots of one call must differ; which token a slot named twice ends up
     with is not defined.
 
     With ``k_weight`` [128], K gets per-head RMSNorm first; with ``frequencies`` [P, R / 2, 2,
     2] (or [1, P, 1, R / 2, 2, 2]; fp32, bf16 or fp16), split-half RoPE of its first R dims by
     row ``positions[t]``, or row t without ``positions``. A position outside the table gives
     NaN in the rotated dims. ``q`` [T, heads, 128] is normalised (``q_weight``) and rotated
-    the same way into ``q_out`` (default: a new tensor; ``q`` itself works in place).
+    the same way into ``q_out`` (default: a new tensor, cleared first; ``q`` itself works in place).
 
     Norm and rotation are fp32 and rounded once, at the store (:func:`h3b200.qknorm_rope_strided_`
     also rounds between the two, as the reference it reproduces does). Returns ``q_out``
@@ -209,7 +209,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             qw = _weight(q_weight, "q_weight", q)
             qw_ptr = qw.data_ptr()
         if q_out is None:
-            q_out = torch.empty_like(q)
+            q_out = torch.zeros_like(q)  # the rows of padding tokens stay as they are
         qoshape, qos = _thd(q_out, "q_out", dtype)
         if qoshape != qshape:
             raise ValueError("q_out must have q's shape")

@@ -1,6 +1,6 @@
 """Edges of the attention operators on the GPU: weights far below their row's largest one, rotation
-tables without rows and outputs made inside a call. References and tolerances as in
-test_gpu_attention.py, where a test says nothing else.
+tables without rows, outputs made inside a call and captured appends. References and tolerances as
+in test_gpu_attention.py, where a test says nothing else.
 """
 
 import math
@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import h3b200
-from test_gpu_attention import D, F64, _gen, attend64, half_step, randn, table, tiny
+from test_gpu_attention import D, F64, _gen, attend64, check_decode, half_step, randn, table, tiny
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +132,62 @@ def test_append_made_q_out_is_zero_for_padding(tokens, heads):
         want = torch.zeros(tokens, heads, D, dtype=torch.bfloat16, device="cuda")
         h3b200.append_paged_kv(k, v, kc, vc, slots, table(tokens, 64), q=q, q_out=want)
         assert torch.equal(out, want)
+
+
+def test_captured_step_follows_slots_tables_and_lengths():
+    """One captured step of append and decode attention, replayed while slots, positions, page_table and lengths
+    change in place: a batch that grows, one sequence of it into pages it did not have at the capture."""
+    gen = _gen(41)
+    b, heads, kv, page, pages, dtype = 3, 8, 2, 16, 40, torch.bfloat16
+    kc, vc = (torch.zeros(pages, kv, page, D, dtype=dtype, device="cuda") for _ in range(2))
+    order = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)
+    tab = torch.full((b, 6), -1, dtype=torch.int32, device="cuda")
+    f, kw = table(256, 96), randn(gen, D, std=0.1) + 1
+    q, k, v = (randn(gen, b, h, D, dtype=dtype) for h in (heads, kv, kv))
+    slots, pos = (torch.full((b,), -1, dtype=torch.int64, device="cuda") for _ in range(2))
+    lens = torch.zeros(b, dtype=torch.int32, device="cuda")
+    q_out = torch.zeros_like(q)
+
+    def step():
+        h3b200.append_paged_kv(k, v, kc, vc, slots, f, pos, k_weight=kw, q=q, q_weight=kw, q_out=q_out)
+        return h3b200.paged_decode_attention(q_out, kc, vc, tab, lens, return_lse=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()      # padding only: nothing is written
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = step()
+    assert not bool(kc.any())
+    seqs = [[], [], []]
+    counts, free = [0, 0, 0], 0
+    for n in range(40):
+        live = [True, n % 3 != 1, n >= 15]       # a sequence rests now and then, one starts late
+        new_slots, new_pos = [-1] * b, [-1] * b
+        for i in range(b):
+            if not live[i]:
+                continue
+            if counts[i] % page == 0:
+                tab[i, counts[i] // page] = order[free]
+                free += 1
+            new_slots[i] = int(tab[i, counts[i] // page]) * page + counts[i] % page
+            new_pos[i] = counts[i] + 7 * i
+            counts[i] += 1
+        q.copy_(randn(gen, b, heads, D, dtype=dtype))
+        k.copy_(randn(gen, b, kv, D, dtype=dtype))
+        v.copy_(randn(gen, b, kv, D, dtype=dtype))
+        slots.copy_(torch.tensor(new_slots))
+        pos.copy_(torch.tensor(new_pos))
+        lens.copy_(torch.tensor(counts, dtype=torch.int32))
+        graph.replay()
+        for i in range(b):
+            if live[i]:
+                at = new_slots[i]
+                seqs[i].append((kc[at // page, :, at % page].clone(), vc[at // page, :, at % page].clone()))
+                assert torch.equal(seqs[i][-1][1], v[i])
+        want, want_lse = h3b200.paged_decode_attention(q_out, kc, vc, tab, lens, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    stacked = [tuple(torch.stack([s[j] for s in seq]) for j in range(2)) for seq in seqs]
+    check_decode(q_out, stacked, out, lse, D ** -0.5, dtype)

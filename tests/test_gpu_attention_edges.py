@@ -1,6 +1,7 @@
 """Edges of the attention operators on the GPU: weights far below their row's largest one, rotation
-tables without rows, outputs made inside a call and captured appends. References and tolerances as
-in test_gpu_attention.py, where a test says nothing else.
+tables without rows, outputs made inside a call, captured appends, and lists and grids longer than
+what the block-sparse kernel reads of them at once. References and tolerances as in
+test_gpu_attention.py, where a test says nothing else.
 """
 
 import math
@@ -9,7 +10,8 @@ import pytest
 import torch
 
 import h3b200
-from test_gpu_attention import D, F64, _gen, attend64, check_decode, half_step, randn, table, tiny
+from test_gpu_attention import (D, F64, _gen, attend64, check_attention, check_decode, half_step, list_mask, randn,
+                                table, tiny)
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +193,50 @@ def test_captured_step_follows_slots_tables_and_lengths():
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
     stacked = [tuple(torch.stack([s[j] for s in seq]) for j in range(2)) for seq in seqs]
     check_decode(q_out, stacked, out, lse, D ** -0.5, dtype)
+
+
+# ---------------------------------------------------------------------------
+# more tiles and items than the block-sparse kernel looks up at once
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries,keys,heads,kv,block,causal", [
+    (2000, 6000, 24, 24, 64, False),      # 47 tiles an item
+    (1300, 9001, 32, 8, 64, False),       # 71
+    (2100, 8500, 20, 4, 128, True),       # up to 67, each query block another count
+])
+def test_sparse_lists_of_many_tiles(dtype, queries, keys, heads, kv, block, causal):
+    """Dense attention through lists of every block: block ids are read 32 tiles at a time."""
+    gen = _gen(queries + keys)
+    q = randn(gen, queries, heads, D, dtype=dtype, std=1.5)
+    k, v = randn(gen, keys, kv, D, dtype=dtype), randn(gen, keys, kv, D, dtype=dtype)
+    top_k = -(-keys // block)
+    out, lse, blocks = h3b200.sparse_attention(q, k, v, top_k, block, causal=causal, return_lse=True, return_blocks=True)
+    for h in (0, heads // 2, heads - 1):
+        g = h // (heads // kv)
+        mask = list_mask(blocks, g, queries, keys, block, causal)
+        ref = attend64(q[:, h], k[:, g], v[:, g], mask, D ** -0.5)
+        check_attention(out[:, h], lse[:, h], ref, dtype, float(v.abs().max()), f"head {h}")
+
+
+@pytest.mark.parametrize("keys,top_k", [(330, 3), (700, 1)])
+def test_sparse_more_items_than_a_stream_looks_up(keys, top_k):
+    """Over 19,000 items on at most 2 streams of each SM: item counts are read 32 at a time."""
+    gen = _gen(keys)
+    queries, heads, kv, dtype = 51201, 48, 4, torch.bfloat16
+    q = randn(gen, queries, heads, D, dtype=dtype, std=1.5)
+    k, v = randn(gen, keys, kv, D, dtype=dtype), randn(gen, keys, kv, D, dtype=dtype)
+    blocks = torch.randint(-2, -(-keys // 64) + 1, (kv, -(-queries // 128), top_k), generator=gen, device="cuda",
+                           dtype=torch.int32)
+    # an id named twice counts twice: the reference's mask cannot say that
+    for i in range(1, top_k):
+        again = (blocks[..., i:i + 1] == blocks[..., :i]).any(-1)
+        blocks[..., i] = torch.where(again, -1, blocks[..., i])
+    out, lse = h3b200.block_sparse_attention(q, k, v, blocks, return_lse=True)
+    for h in (0, 5, 23, 47):
+        g = h // (heads // kv)
+        ref = attend64(q[:, h], k[:, g], v[:, g], list_mask(blocks, g, queries, keys, 64, False), D ** -0.5)
+        check_attention(out[:, h], lse[:, h], ref, dtype, float(v.abs().max()), f"head {h}")
+    out2, lse2 = h3b200.block_sparse_attention(q, k, v, blocks, return_lse=True)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)

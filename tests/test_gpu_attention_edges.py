@@ -86,6 +86,32 @@ def test_sparse_keeps_faint_weights(dtype, t, n, heads, kv):
         check_faint(out[rows, h], lse[rows, h], q[rows, h], k[:, g], v[:, g], smallest)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("top", [700.0, 2000.0])
+def test_scores_of_many_millions_pick_one_key(dtype, top):
+    """Where scores are so large that fp32 holds no fraction of them, a row is its best key's value: off by the
+    rounding of one weight and of the result. Every row has another maximum, so that its rounding goes either way."""
+    gen = _gen(int(top))
+    n, best, rows = 100, 70, 200
+    v = randn(gen, n, 1, D, dtype=dtype)
+    size = torch.linspace(0.25 * top, top, rows, device="cuda").to(dtype)
+    k = (0.9 * top * torch.rand(n, 1, 1, generator=gen, device="cuda")).expand(n, 1, D).to(dtype).contiguous()
+    k[best] = top
+    q = size[:, None, None].expand(rows, 1, D).contiguous()
+    score = D * size.to(F64) * float(k[best, 0, 0]) * D ** -0.5
+    page = 8
+    pad = torch.zeros(104 - n, 1, D, dtype=dtype, device="cuda")
+    kc, vc = (torch.cat((x, pad)).reshape(13, page, 1, D).transpose(1, 2) for x in (k, v))
+    tab = torch.arange(13, dtype=torch.int32, device="cuda").expand(rows, 13)
+    lens = torch.full((rows,), n, dtype=torch.int32, device="cuda")
+    for out, lse in (h3b200.paged_decode_attention(q, kc, vc, tab, lens, return_lse=True),
+                     h3b200.sparse_attention(q, k, v, 2, return_lse=True)):
+        off = (out[:, 0].to(F64) - v[best, 0].to(F64)).abs()
+        assert bool((off <= 2.01 * half_step(dtype) * v[best, 0].to(F64).abs() + tiny(dtype)).all())
+        # the fp32 sum of 128 equal products is off by at most 128 * 2^-24 of it
+        assert bool(((lse[:, 0].to(F64) - score).abs() <= 130 * 2.0 ** -24 * score).all())
+
+
 # ---------------------------------------------------------------------------
 # append
 # ---------------------------------------------------------------------------

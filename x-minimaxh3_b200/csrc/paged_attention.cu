@@ -197,6 +197,9 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
       }
       if (g >= valid[0]) s[0] = s[1] = -INFINITY;
       if (g >= valid[1]) s[2] = s[3] = -INFINITY;
+      // Weights and rescaling are taken of differences to the maximum: with one fused
+      // multiply-add of the score and the scaled maximum, the rounding of that maximum is
+      // the largest weight's exponent, and fp16 overflows from scores of 1e7 on.
       float f[2], sub[2];
       bool grew = false;
 #pragma unroll
@@ -206,8 +209,8 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
         const float mn = fmaxf(m[n][e], mx);
-        sub[e] = mn == -INFINITY ? 0.0f : mn * p.scale_log2;
-        f[e] = exp2f(m[n][e] * p.scale_log2 - sub[e]);  // exp2(-inf) = 0 before the first key
+        sub[e] = mn == -INFINITY ? 0.0f : mn;
+        f[e] = mn == m[n][e] ? 1.0f : exp2f((m[n][e] - mn) * p.scale_log2);  // exp2(-inf) = 0 before the first key
         grew = grew || mn > m[n][e];
         m[n][e] = mn;
       }
@@ -224,7 +227,7 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? 3 : 2) paged_decode_ker
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[e] = exp2f(fmaf(s[e], p.scale_log2, DecodeWeight<F16>::log2 - sub[e & 1]));
+        s[e] = exp2f(fmaf(s[e] - sub[e & 1], p.scale_log2, DecodeWeight<F16>::log2));
         l[n][e & 1] += s[e];
       }
       pb[n][0] = movmatrix_trans(E::pack(s[0], s[1]));

@@ -531,14 +531,18 @@ __global__ void __launch_bounds__(kSpThreads, 1)
         uint64_t sum[2];
 #pragma unroll 1
         for (;;) {
-          const float sub = m == -INFINITY ? 0.0f : m * p.scale_log2;
-          const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), sub2 = f2_pack(SparseWeight<F16>::log2 - sub, SparseWeight<F16>::log2 - sub);
+          // in fp16 rounded down: from scores of 1e7 on, rounding to nearest is whole powers
+          // of 2, which must not lift the largest weight over 65,504
+          const float shift = m == -INFINITY ? SparseWeight<F16>::log2
+                              : F16          ? __fmaf_rd(-m, p.scale_log2, SparseWeight<F16>::log2)
+                                             : -(m * p.scale_log2);
+          const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2), shift2 = f2_pack(shift, shift);
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
           sum[0] = sum[1] = 0ull;
 #pragma unroll
           for (int e = 0; e < 32; ++e) {
             const float y0 = __uint_as_float(x[e >> 4][2 * (e & 15)]), y1 = __uint_as_float(x[e >> 4][2 * (e & 15) + 1]);
-            const uint64_t z = f2_fma(f2_pack(y0, y1), scale2, sub2);
+            const uint64_t z = f2_fma(f2_pack(y0, y1), scale2, shift2);
             float a, b;
             if (e % kPolyOf == kPolyOf - 1) {
               exp2_poly2(z, a, b);

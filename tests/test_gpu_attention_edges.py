@@ -266,3 +266,105 @@ def test_sparse_more_items_than_a_stream_looks_up(keys, top_k):
         check_attention(out[:, h], lse[:, h], ref, dtype, float(v.abs().max()), f"head {h}")
     out2, lse2 = h3b200.block_sparse_attention(q, k, v, blocks, return_lse=True)
     assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+# ---------------------------------------------------------------------------
+# what the documentation allows
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("queries,keys,heads,kv,top_k,causal", [
+    (1, 700, 40, 2, 4, False),         # the decode kernel: two row tiles
+    (1, 9000, 8, 2, 141, False),
+    (200, 3000, 4, 2, 47, True),       # split lists, joined by a second kernel
+    (2500, 2500, 24, 24, 5, True),
+])
+def test_sparse_output_in_place_of_the_queries(queries, keys, heads, kv, top_k, causal):
+    gen = _gen(queries + top_k)
+    q = randn(gen, queries, heads, D, std=1.5)
+    k, v = randn(gen, keys, kv, D), randn(gen, keys, kv, D)
+    want, lse, blocks = h3b200.sparse_attention(q, k, v, top_k, causal=causal, return_lse=True, return_blocks=True)
+    mine = q.clone()
+    got, lse2, blocks2 = h3b200.sparse_attention(mine, k, v, top_k, causal=causal, out=mine, return_lse=True,
+                                                 return_blocks=True)
+    assert got is mine and torch.equal(got, want) and torch.equal(lse, lse2) and torch.equal(blocks, blocks2)
+    mine = q.clone()
+    assert torch.equal(h3b200.block_sparse_attention(mine, k, v, blocks, causal=causal, out=mine), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("queries", [1, 300, 900])
+def test_packed_projection_rows_and_kept_means(dtype, queries):
+    """q, k, v as slices of packed projection rows, out as a slice of wider rows, k_means as a slice of a longer
+    buffer: the same bits as from tensors of their own."""
+    gen = _gen(queries)
+    heads, kv, keys = 12, 4, 900
+    x = randn(gen, keys, (heads + 2 * kv) * D, dtype=dtype)
+    q, k, v = (y.reshape(keys, -1, D) for y in x.split((heads * D, kv * D, kv * D), 1))
+    q = q[keys - queries:]
+    wide = torch.zeros(queries, 2 * heads * D, dtype=dtype, device="cuda")
+    out = wide[:, heads * D:].reshape(queries, heads, D)
+    means = torch.full((kv, 40, D), float("nan"), device="cuda")
+    means[:, :15] = h3b200.attention_block_means(k, 64)
+    got, lse = h3b200.sparse_attention(q, k, v, 6, causal=True, k_means=means[:, :15], out=out, return_lse=True)
+    want, lse2, blocks = h3b200.sparse_attention(q.contiguous(), k.contiguous(), v.contiguous(), 6, causal=True,
+                                                 return_lse=True, return_blocks=True)
+    assert torch.equal(got, want) and torch.equal(lse, lse2) and not bool(wide[:, :heads * D].any())
+    for h in (0, heads - 1):
+        g = h // (heads // kv)
+        ref = attend64(q[:, h], k[:, g], v[:, g], list_mask(blocks, g, queries, keys, 64, True), D ** -0.5)
+        check_attention(out[:, h], lse[:, h], ref, dtype, float(v.abs().max()), f"head {h}")
+
+
+@pytest.mark.parametrize("queries", [1, 260])
+@pytest.mark.parametrize("block", [64, 128])
+def test_blocks_named_twice_count_twice(queries, block):
+    gen = _gen(queries + block)
+    heads, keys, dtype = 2, 1000, torch.bfloat16
+    q, k, v = (randn(gen, n, heads, D, dtype=dtype) for n in (queries, keys, keys))
+    ids = torch.tensor([2, 5, 2, -1, 7, 5, 5], dtype=torch.int32, device="cuda")
+    blocks = ids.expand(heads, -(-queries // 128), 7).contiguous()
+    out, lse = h3b200.block_sparse_attention(q, k, v, blocks, block, return_lse=True)
+    at = torch.cat([torch.arange(i * block, min(keys, (i + 1) * block), device="cuda") for i in ids.tolist()
+                    if 0 <= i < -(-keys // block)])
+    mask = torch.ones(queries, at.numel(), dtype=torch.bool, device="cuda")
+    for h in range(heads):
+        ref = attend64(q[:, h], k[at, h], v[at, h], mask, D ** -0.5)
+        check_attention(out[:, h], lse[:, h], ref, dtype, float(v.abs().max()), f"head {h}")
+
+
+def test_calls_at_once_on_two_streams():
+    """Two streams, each with its own calls of every operator, some with workspaces and joins: the same bits as alone."""
+    gen = _gen(51)
+    dtype, kv, page = torch.bfloat16, 2, 32
+    jobs = []
+    for n, t in ((30000, 200), (5000, 1500)):
+        pages = -(-n // page)
+        kc, vc = (randn(gen, pages, kv, page, D) for _ in range(2))
+        tab = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)[None]
+        lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+        q1, qs = randn(gen, 1, 8, D), randn(gen, t, 8, D)
+        k, v = randn(gen, n, kv, D), randn(gen, n, kv, D)
+        slots = torch.arange(t, device="cuda")
+        f, kw = table(t, 64), randn(gen, D)
+
+        def job(kc=kc, vc=vc, tab=tab, lens=lens, q1=q1, qs=qs, k=k, v=v, slots=slots, f=f, kw=kw, t=t):
+            a = h3b200.paged_decode_attention(q1, kc, vc, tab, lens, return_lse=True)
+            b = h3b200.sparse_attention(qs, k, v, 20, causal=True, return_lse=True, return_blocks=True)
+            c = h3b200.sparse_attention(q1, k, v, 33)
+            kn, vn = torch.zeros_like(kc), torch.zeros_like(vc)
+            d = h3b200.append_paged_kv(k[:t], v[:t], kn, vn, slots, f, k_weight=kw, q=qs)
+            return (*a, *b, c, kn, vn, d)
+
+        jobs.append(job)
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(20):
+        got = []
+        for s, job in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(job())
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -368,3 +368,20 @@ def test_calls_at_once_on_two_streams():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_one_page_of_more_than_a_million_keys():
+    """A cache without paging is one long page per sequence."""
+    gen = _gen(61)
+    page, n, heads, dtype = (1 << 20) + 8, 5000, 4, torch.bfloat16
+    kc, vc = (torch.zeros(2, 1, page, D, dtype=dtype, device="cuda") for _ in range(2))
+    k, v = randn(gen, n, 1, D), randn(gen, n, 1, D)
+    slots = page + (page - n) + torch.arange(n, device="cuda")     # the second page's last rows
+    h3b200.append_paged_kv(k, v, kc, vc, slots)
+    assert torch.equal(kc[1, 0, page - n:], k[:, 0]) and torch.equal(vc[1, 0, page - n:], v[:, 0])
+    assert not bool(kc[0].any()) and not bool(kc[1, :, :page - n].any())
+    q = randn(gen, 1, heads, D)
+    tab = torch.tensor([[1]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([page], dtype=torch.int32, device="cuda")
+    out, lse = h3b200.paged_decode_attention(q, kc, vc, tab, lens, return_lse=True)
+    check_decode(q, [(kc[1].transpose(0, 1), vc[1].transpose(0, 1))], out, lse, D ** -0.5, dtype)

@@ -1440,8 +1440,8 @@ constexpr int64_t kMaxKeys = 1 << 30;  // key indices of one sequence are 32-bit
 
 // page sizes are multiples of 8 keys
 int paged_shape(int64_t pages, int64_t page_size, const char* who) {
-  if (pages >= 0 && page_size > 0 && page_size % 8 == 0 && page_size <= (1 << 20)) return H3B200_OK;
-  return fail(H3B200_ERR_INVALID, "%s: page_size must be a positive multiple of 8 (got %lld) and pages >= 0 (got %lld)", who, (long long)page_size, (long long)pages);
+  if (pages >= 0 && page_size > 0 && page_size % 8 == 0 && page_size <= kMaxKeys) return H3B200_OK;
+  return fail(H3B200_ERR_INVALID, "%s: page_size must be a positive multiple of 8, at most 2^30 (got %lld) and pages >= 0 (got %lld)", who, (long long)page_size, (long long)pages);
 }
 
 }  // namespace

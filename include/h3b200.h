@@ -627,7 +627,13 @@ H3B200_API int h3b200_tp_gated_mlp(void* comm, const void* x, int64_t ldx, const
  * H3B200_DTYPE_F16, one for all tensors of a call. head_dim is 128. Strides are in
  * elements, multiples of 8; the head dim is contiguous and rows are 16-byte
  * aligned. Sums, softmax statistics, norms and rotations are fp32 (block means and
- * their products 64-bit); results are rounded once, when they are stored.
+ * their products 64-bit) and results are rounded when they are stored. Softmax weights
+ * are rounded before that too, to the element type, as the tensor core's operand in
+ * the product with V (their sum takes them unrounded): a result is off by up to half a
+ * step of the type for the weights, half a step for itself. In fp16 the weights are held
+ * times a power of 2, so that those down to 2^-32 (block-sparse) or 2^-40 (decode) of a
+ * row's largest count. Scores (scale q.k) beyond 1e8, of which fp32 holds no fraction,
+ * are outside the contract.
  * The reference runs attention through external libraries (kernels.py:7637); these
  * entry points have no counterpart in it.
  * ---------------------------------------------------------------------- */
@@ -667,7 +673,8 @@ H3B200_API int h3b200_append_paged_kv(const void* q, int64_t q_st, int64_t q_sh,
  * key head h / (heads / kv_heads). lengths (int32) are clamped to [0, table_width *
  * page_size]; a sequence without keys gives 0 and lse = -inf. Page ids outside
  * [0, pages) hold no keys (nothing is read). Rows behind a sequence's last key are not
- * read into the result, whatever they hold. page_size: a multiple of 8. page_table:
+ * read into the result, whatever they hold. page_size: a multiple of 8, table_width *
+ * page_size at most 2^30. page_table:
  * int32 [batch, table_width] at stride pt_sb. out, lse strides as given.
  * workspace: h3b200_paged_decode_workspace_bytes (which depends on the current device's SM
  * count) bytes, 256-byte aligned; not needed after the call's work has run.
@@ -700,7 +707,12 @@ H3B200_API int h3b200_attention_block_means(const void* x, int64_t x_st, int64_t
  * lowest j; NaN below every number), -1 behind them when fewer blocks can be seen.
  * causal: query row r stands at position r + keys - queries. Key blocks that start
  * behind the query block's last position are never selected; those that hold a
- * position at or behind its first one come before all others.
+ * position at or behind its first one come before all others, the lowest first: with a
+ * top_k below their number (2 or 3 blocks of 64, 1 or 2 of 128) the query block's last
+ * rows do not see their own positions.
+ * Scores are off by about 1e-16 of the sum of their terms' sizes. Blocks whose scores
+ * differ by less can change places; those with equal means never do. At most 24,556 key
+ * blocks are built.
  */
 H3B200_API int h3b200_select_key_blocks(const float* q_means, const float* k_means, int64_t km_sh, int64_t km_sb,
                                         int64_t heads, int64_t kv_heads, int64_t queries, int64_t keys, int64_t block,
@@ -715,7 +727,8 @@ H3B200_API int h3b200_select_key_blocks(const float* q_means, const float* k_mea
  * key gives 0 and lse = -inf. block: 64 or 128 keys. Values of a tile that some row of a
  * query block may not see (causal) still enter its products with weight zero, so they
  * must be finite; rows behind the last key do not exist for the kernel. q, k, v, out:
- * [tokens, heads, 128] at token / head strides. scale > 0.
+ * [tokens, heads, 128] at token / head strides, positive ones for q, k and v where
+ * queries > 1 (a broadcast dim has no tensor map). out may be q. scale > 0.
  * workspace: h3b200_block_sparse_workspace_bytes (which depends on the current device's SM
  * count) bytes, 256-byte aligned; not needed after the call's work has run.
  */

@@ -6,8 +6,8 @@
 // table[j / page_size]. A sequence without keys gives 0 and lse = -inf.
 //
 // Bound: HBM. Every key and value row is read once for the whole group of query
-// heads that share it, 4 bytes per two multiply-adds and head, so the kernel
-// only has to keep enough loads in flight. One warp takes 16 keys at a time and
+// heads that share it (groups of more than 16 heads load it once per 16 heads), 4 bytes
+// per two multiply-adds and head, so the kernel only has to keep enough loads in flight. One warp takes 16 keys at a time and
 // reads them straight into matrix-instruction operands; nothing is staged in
 // shared memory:
 //  * S^T = K Q^T (16 keys x 8 query heads, m16n8k16). The contraction index can
@@ -23,8 +23,8 @@
 // The small M of this work (the group's 1 to 16 heads) would leave a tcgen05
 // tile of 128 rows almost empty, and staging through shared memory for it would
 // cost what the direct loads save. Measured: 64 sequences of 8,192 keys, 8 key heads
-// (2.15 GB): 337 us, 97% of the measured copy bandwidth; one of 250,001 keys, 4 key heads
-// (0.51 GB): 90 us, 87%.
+// (2.15 GB): 336 us, 98% of the measured copy bandwidth; one of 250,001 keys, 4 key heads
+// (0.51 GB): 85 to 89 us, 88 to 92%.
 //
 // The length of a sequence is split over CTAs, each with its own m, l and unnormalised O.
 // Up to 8 splits are one cluster, where all CTAs fit on the GPU at once: they write theirs
@@ -412,7 +412,9 @@ constexpr int kPartMin = 64;     // keys: one 16-key step of each warp
 constexpr int kPartGood = 512;   // keys whose reading outweighs a part's own cost by far
 // Parts of each sequence where the items alone fill the GPU: 64 x 8 key heads of 7,000 to
 // 9,000 keys take 330 us in 4, 338 in 8, 358 in 12 parts; 48 x 8 of 0 to 6,000 keys 114,
-// 113 and 123.
+// 113 and 123. The number of parts comes from the shape alone, so one long sequence
+// among short ones runs on its few parts long after the others have ended: 250,001 keys
+// beside 63 sequences of 100 to 2,000 take 1,476 us, where the bytes alone take 199.
 constexpr int kTailParts = 4;
 constexpr int kMaxSplits = 512;
 constexpr int kClusterMax = 8;   // portable cluster size

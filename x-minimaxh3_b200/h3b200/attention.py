@@ -7,6 +7,11 @@ contract, ``NotImplementedError`` for valid ones that are not built, no fallback
 are bf16 or fp16 (one type for all tensors of a call), the head dim is 128. The operators
 are for inference: they record nothing for autograd.
 
+Scores, sums and softmax statistics of the attention operators are fp32. The softmax
+weights are rounded to the element type for the product with V (the tensor core's
+operand), beside the rounding of the result: the worst error of a result is about twice
+that of one rounding.
+
 A call on one token is bound by the host, so each operator asks a tensor for its shape,
 strides and type once and makes one call into the library.
 """
@@ -231,7 +236,8 @@ def paged_decode_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     """Attention of one new token per sequence over the pages :func:`append_paged_kv` fills.
 
     ``q`` [B, heads, 128]; ``k_cache`` / ``v_cache`` [pages, kv_heads, page_size, 128]
-    (page_size a multiple of 8, heads a multiple of kv_heads); ``page_table`` int32 [B, width]:
+    (page_size a multiple of 8, width * page_size at most 2^30, heads a multiple of
+    kv_heads); ``page_table`` int32 [B, width]:
     key j of sequence b is row ``j % page_size`` of page ``page_table[b, j // page_size]``;
     ``lengths`` int32 [B]: keys of each sequence, the new token's own among them (clamped to
     what the table holds). ``scale`` defaults to 1 / sqrt(128).
@@ -313,10 +319,13 @@ def select_key_blocks(q_means: torch.Tensor, k_means: torch.Tensor, top_k: int, 
     Row i of a key head holds the ``top_k`` blocks j with the highest ``q_means[h, i] .
     k_means[kv_head, j]``, summed over the query heads h of the group, in ascending order
     (equal scores: the lowest j), and -1 behind them when it can see fewer. Scores are held
-    in 64 bits, so that the selection does not depend on a summation order.
+    in 64 bits: another summation order changes a selection only where two scores agree to
+    about 1e-16 of their terms. At most 24,556 key blocks are built.
 
     ``causal``: query row r stands at position ``r + keys - queries``. Blocks that start
-    behind the query block are never selected, and those that reach into it come first."""
+    behind the query block are never selected, and those that reach into it come first, the
+    lowest of them before the others: with ``top_k`` below their number (up to 3 blocks of
+    64, 2 of 128) the last rows do not see their own positions."""
     dev = _device(q_means, k_means)
     queries, keys, block_size, top_k = int(queries), int(keys), int(block_size), int(top_k)
     if queries < 0 or keys < 0 or not 0 < block_size <= 1 << 20 or not 0 < top_k <= 1 << 24:
@@ -371,7 +380,8 @@ def block_sparse_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, bl
     """Attention of 128-row query blocks over the key blocks ``blocks`` lists.
 
     ``q`` [T, heads, 128], ``k`` / ``v`` [S, kv_heads, 128] (any token and head strides, e.g.
-    HND-backed views); ``blocks`` int32 [kv_heads, ceil(T / 128), top_k] as
+    HND-backed views; expanded dims, of stride 0, are not built for more than one query);
+    ``blocks`` int32 [kv_heads, ceil(T / 128), top_k] as
     :func:`select_key_blocks` returns it: ids outside the keys' blocks (-1) name none, an id
     named twice counts twice. ``block_size`` is 64 or 128 keys. With ``causal``, query row r
     sees the listed keys at positions up to ``r + S - T``. A row that sees no key gives
